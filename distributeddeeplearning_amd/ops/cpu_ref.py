@@ -224,6 +224,94 @@ def dense1_bce_fwd_bwd(x, w, b, label_first: float, label_second: float, n_first
     return loss, dx, dw, db, logits
 
 
+def dense_softmax_ce(x, w, bias, labels, want_grad: bool = True):
+    """Dense + softmax cross entropy with integer labels; rows with a negative label are left out.
+    Returns (loss, dx, dw, db, rows)."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"dense_softmax_ce: x {tuple(x.shape)} and w {tuple(w.shape)} must be [N][K] and [V][K]")
+    N, V = x.shape[0], w.shape[0]
+    if labels.dtype != torch.int64 or labels.numel() != N:
+        raise ValueError(f"labels must be an int64 vector of {N} class numbers")
+    if bias is not None and bias.numel() != V:
+        raise ValueError(f"bias: {bias.numel()} elements, need {V}")
+    live = (labels >= 0) & (labels < V)
+    count = (labels >= 0).sum().clamp_min(1).float()
+    xf = torch.where(live[:, None], x.float(), torch.zeros(()))
+    wf = w.float()
+    z = xf @ wf.t()
+    if bias is not None:
+        z = z + bias.float()
+    at = torch.where(live, labels, torch.zeros_like(labels))[:, None]
+    lse = torch.logsumexp(z, 1)
+    bad = ~torch.isfinite(lse)
+    rows = torch.where(bad, torch.full_like(lse, math.nan), lse - z.gather(1, at)[:, 0])
+    rows = torch.where(live, rows, torch.where(labels < 0, torch.zeros_like(rows), torch.full_like(rows, math.nan)))
+    loss = rows.double().sum().div(count.double()).float()
+    if not want_grad:
+        return loss, None, None, None, rows
+    dl = torch.exp(z - lse[:, None])
+    dl.scatter_add_(1, at, torch.full_like(at, -1, dtype=dl.dtype))
+    dl = torch.where(bad[:, None], torch.full_like(dl, math.nan), dl / count)
+    dl = torch.where(live[:, None], dl, torch.zeros(()))
+    return loss, dl @ wf, dl.t() @ xf, (dl.sum(0) if bias is not None else None), rows
+
+
+# --------------------------------------------------------------------------- 8-bit activation checkpoints
+def pack8(x):
+    """Blocks of 32 elements in memory order: e = smallest integer in -119 .. 121 with max |x| <= 127 2^e, code = x 2^-e
+    rounded to the nearest integer (ties to even), +-1 where a non-zero x would get 0."""
+    from .functional import Packed8
+    flat = x.float().contiguous().reshape(-1)
+    n = flat.numel()
+    nb = (n + 31) // 32
+    blk = F.pad(flat, (0, nb * 32 - n)).view(nb, 32)
+    bad = ~torch.isfinite(blk).all(1)
+    blk = torch.where(bad[:, None], torch.zeros(()), blk)
+    mant, exp = torch.frexp(blk.abs().amax(1)) if nb else (torch.empty(0), torch.empty(0, dtype=torch.int32))
+    e = torch.where(mant * 128 <= 127, exp - 7, exp - 6).clamp(-119, 121)
+    e = torch.where(mant == 0, torch.full_like(e, -119), e)
+    q = torch.round(torch.ldexp(blk.double(), -e[:, None])).clamp(-127, 127)
+    q = torch.where((q == 0) & (blk != 0), torch.sign(blk).double(), q)
+    return Packed8(q.reshape(-1)[:n].to(torch.int8).view(x.shape),
+                   torch.where(bad, torch.full_like(e, 255), e + 127).to(torch.uint8))
+
+
+def unpack8(q, out=None):
+    s = torch.ldexp(torch.ones(q.scales.shape, dtype=torch.float64), q.scales.int() - 127)
+    s = torch.where(q.scales == 255, torch.full_like(s, math.nan), s).float()
+    y = (q.codes.reshape(-1).float() * s.repeat_interleave(32)[:q.codes.numel()]).view(q.codes.shape)
+    if out is None:
+        return y
+    if out.numel() != y.numel():
+        raise ValueError(f"out: {out.numel()} elements, need {y.numel()}")
+    return out.copy_(y.reshape(out.shape))
+
+
+def act_bwd8(dy, q, kind, alpha: float = 0.3):
+    if kind in (None, "linear"):
+        return dy
+    if dy.shape != q.codes.shape:
+        raise ValueError(f"act_bwd8: dy {tuple(dy.shape)}, checkpoint {tuple(q.codes.shape)}")
+    y = unpack8(q)
+    return act_bwd(dy, y, kind, alpha) + torch.where(y == y, torch.zeros(()), torch.full((), math.nan))
+
+
+def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
+    if q.codes.dim() != 2 or dy.dim() != 2 or q.codes.shape[0] != dy.shape[0]:
+        raise ValueError(f"dense_wgrad8: checkpoint {tuple(q.codes.shape)} and dy {tuple(dy.shape)} must be [R][K] and [R][O]")
+    O = dy.shape[1] if n_out is None else int(n_out)
+    if not 0 < O <= dy.shape[1]:
+        raise ValueError(f"dense_wgrad8: {O} outputs of {dy.shape[1]}")
+    d = dy.float()[:, :O]
+    dw, db = d.t() @ unpack8(q), d.sum(0)
+    for t, o in ((dw, out_dw), (db, out_db)):
+        if o is not None:
+            if o.numel() != t.numel():
+                raise ValueError(f"output: {o.numel()} elements, need {t.numel()}")
+            o.copy_(t.reshape(o.shape))
+    return (dw if out_dw is None else out_dw), (db if out_db is None else out_db)
+
+
 # --------------------------------------------------------------------------- metrics / data
 def argmax_match_count(pred, onehot):
     return (pred.float().argmax(-1) == onehot.float().argmax(-1)).sum()

@@ -241,5 +241,87 @@ def dense1_bce_fwd_bwd(x, w, b, label_first, label_second, n_first, want_dx=True
     return loss, dx, dw, db, logits
 
 
+def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):
+    """Dense(K -> V) + softmax cross entropy for any number of classes, forward and backward, without the logits.
+
+    x [N][K], w [V][K] (device: bf16, K padded to a multiple of 8 with zero lanes), bias [V] fp32 or None (-inf switches
+    a class off), labels [N] int64.  A row whose label is negative takes no part, whatever its x holds: row loss 0, dx 0,
+    not counted.  Returns (loss, dx, dw, db, rows): the mean over the labelled rows (0 if there are none), the gradients
+    of that mean (None without `want_grad`; db None without a bias) and the row losses.  dx has x's type, dw [V][K] and
+    db [V] `grad_dtype` (fp32 | bf16), or they overwrite `out_dw` / `out_db` in those tensors' type.
+
+    A label past the last class makes its row loss (and the mean) NaN and its row no gradient; a labelled row with a NaN
+    or infinite logit, or with every class switched off, has NaN loss and gradients.  On the device the gradient of the
+    logits is rounded to bf16 as every dY is, twice for dw (its scale is folded into x)."""
+    if x.is_cuda:
+        return hip_backend().dense_softmax_ce(x, w, bias, labels, want_grad, out_dw, out_db, grad_dtype)
+    loss, dx, dw, db, rows = cpu_ref.dense_softmax_ce(x, w, bias, labels, want_grad)
+    if want_grad:
+        dw, db = (_cpu_out(t, o, grad_dtype) for t, o in ((dw, out_dw), (db, out_db)))
+    elif out_dw is not None or out_db is not None:
+        raise ValueError("dense_softmax_ce: out_dw / out_db need want_grad")
+    return loss, dx, dw, db, rows
+
+
+def _cpu_out(t, out, dtype):
+    if out is None:
+        return t if t is None else t.to(dtype)
+    if t is None:
+        raise ValueError("an output tensor for a gradient that is not computed")
+    if out.numel() != t.numel():
+        raise ValueError(f"output: {out.numel()} elements, need {t.numel()}")
+    out.copy_(t.reshape(out.shape))
+    return out
+
+
+# 8-bit activation checkpoints ----------------------------------------------------------------
+class Packed8:
+    """An activation tensor in 8 bits: `codes` (int8, the tensor's shape) and `scales` (uint8, one per 32 consecutive
+    codes in memory order, exponent + 127; 255: the block held a NaN or an infinity and reads as NaN).  The value of a
+    code is code * 2^(scale - 127), exact in bf16."""
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise ValueError(f"Packed8: int8 codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+        if scales.numel() != (codes.numel() + 31) // 32:
+            raise ValueError(f"Packed8: {codes.numel()} codes need {(codes.numel() + 31) // 32} scales, got {scales.numel()}")
+        self.codes, self.scales = codes, scales
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    def reshape(self, *shape):
+        return Packed8(self.codes.reshape(*shape), self.scales)
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def pack8(x):
+    """Activation tensor -> Packed8 (33 bytes per 32 elements).  Per 32 elements the scale is the smallest power of two
+    from 2^-119 to
+    2^121 with max |x| <= 127 scale; codes round to nearest even, except that no non-zero value becomes 0 and the largest
+    bf16 number stays finite."""
+    return _b(x).pack8(x)
+
+
+def unpack8(q, out=None):
+    """Packed8 -> activation tensor (device: bf16, exact; CPU: fp32)."""
+    return (hip_backend() if q.codes.is_cuda else cpu_ref).unpack8(q, out)
+
+
+def act_bwd8(dy, q, kind, alpha=0.3):
+    """Activation backward dx = dy * act'(y) with y = act(x) read from its 8-bit checkpoint."""
+    return _b(dy).act_bwd8(dy, q, kind, alpha)
+
+
+def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
+    """Gradients of a Dense layer's weights [O][K] and bias [O] (fp32) from its input's 8-bit checkpoint [R][K] and
+    dy [R][Op]; `n_out`: O, when dy carries padding lanes behind it."""
+    return _b(dy).dense_wgrad8(q, dy, out_dw, out_db, n_out)
+
+
 def argmax_match_count(pred, onehot):
     return _b(pred).argmax_match_count(pred, onehot)

@@ -2399,3 +2399,253 @@ def conv_wgrad(x, dy, g: ConvGeom, layout="A", out=None, box=None, x_affine=None
         raise ValueError(f"conv_wgrad rejected the problem (rc={rc}): {g}")
     _done()
     return out
+
+
+# ------------------------------------------------------------------------------ wide softmax head
+_ce_stats_cols = _sig("ddl_ce_stats_cols", ci, ci, ci)
+_ce_logits = _sig("ddl_ce_logits", ci, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, ci, vp, ci, vp)
+_ce_rows = _sig("ddl_ce_rows", ci, vp, ci, ci, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, vp, vp, ci, vp)
+_ce_mean = _sig("ddl_ce_mean", ci, vp, vp, ci, vp, vp)
+_ce_dx = _sig("ddl_ce_dx", ci, vp, vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, ci, vp)
+_ce_dw = _sig("ddl_ce_dw", ci, vp, vp, ci, ci, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, vp)
+
+# Workspace of a training call in bytes: the exponentials of one piece of rows, 2 bytes per row and class.  4 GiB is
+# 8192 rows of 262144 classes and 1.4 % of the card's memory; a piece costs one more pass over the fp32 weight gradient.
+CE_PIECE_BYTES = int(os.environ.get("DDL_CE_PIECE_BYTES", str(4 << 30)))
+_CE_WAVE_COLS = {0: 128, 1: 64, 2: 32, 3: 16}
+
+
+def _rc(rc, what):
+    if rc != 0:
+        raise RuntimeError(f"{what}: kernel launch refused (code {rc})")
+
+
+def _on_device(t):
+    """Launches go to the current device's current stream: make the tensors' device the current one."""
+    return torch.cuda.device(t.device)
+
+
+def _chk_out(t, n, dtypes, like, name):
+    if not (t.device == like.device and t.dtype in dtypes and t.is_contiguous() and t.numel() == n):
+        raise ValueError(f"{name}: need a contiguous tensor of {n} elements, {' / '.join(map(str, dtypes))} on {like.device}, "
+                         f"got {tuple(t.shape)} {t.dtype} {t.device} contiguous={t.is_contiguous()}")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name}: not 16-byte aligned")
+
+
+def _ce_logits_tile(n, V):
+    """Rows x classes of a tile: as few padding rows as the batch leaves, and enough blocks for 256 CUs."""
+    if n <= 32:
+        return 3 if V < 256 * 128 else 2
+    if n <= 128 or ceil_div(V, 256) * ceil_div(n, 256) < 256:
+        return 1
+    return 0
+
+
+def ceil_div(a, b):
+    return -(-a // b)
+
+
+def _ce_split(V, tiles, want):
+    """(splits, classes per split): the reduction over the classes is cut until `want` blocks run."""
+    steps = ceil_div(V, 64)
+    ns = max(1, min(want // max(tiles, 1), steps // 4, 64))
+    per = ceil_div(steps, ns) * 64
+    return ceil_div(V, per), per
+
+
+def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):
+    """Dense(K -> V) + softmax cross entropy (csrc/hip/dense_ce.hip).  x [N][Kp] bf16, w [V][Kp] bf16, bias [V] fp32
+    or None, labels [N] int64 (negative: row left out).  Returns (loss, dx, dw, db, rows)."""
+    _chk_act(x, "x")
+    _chk_act(w, "w")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"dense_softmax_ce: x {tuple(x.shape)} and w {tuple(w.shape)} must be [N][K] and [V][K]")
+    N, K = x.shape
+    V = w.shape[0]
+    dev = x.device
+    if V < 1 or K < 8 or max(N, V) >= 1 << 28 or K >= 1 << 22:
+        raise ValueError(f"dense_softmax_ce: N={N} K={K} V={V} outside the supported range")
+    for t, name in ((w, "w"), (bias, "bias"), (labels, "labels"), (out_dw, "out_dw"), (out_db, "out_db")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"dense_softmax_ce: {name} is on {t.device}, x on {dev}")
+    if bias is not None:
+        _chk_f32(bias, V, "bias")
+        if bias.numel() != V:
+            raise ValueError(f"bias: {bias.numel()} elements, need {V}")
+    if labels.dtype != torch.int64 or not labels.is_contiguous() or labels.numel() != N:
+        raise ValueError(f"labels must be a contiguous int64 vector of {N} class numbers")
+    dw = db = dx = None
+    if want_grad:
+        if out_dw is not None:
+            grad_dtype = out_dw.dtype
+        elif out_db is not None:
+            grad_dtype = out_db.dtype
+        if grad_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"dense_softmax_ce: gradients are fp32 or bf16, not {grad_dtype}")
+        dw = torch.empty(V, K, dtype=grad_dtype, device=dev) if out_dw is None else out_dw
+        _chk_out(dw, V * K, (grad_dtype,), x, "out_dw")
+        if bias is not None:
+            db = torch.empty(V, dtype=grad_dtype, device=dev) if out_db is None else out_db
+            _chk_out(db, V, (grad_dtype,), x, "out_db")
+        elif out_db is not None:
+            raise ValueError("dense_softmax_ce: out_db without a bias")
+        dx = torch.empty_like(x)
+    elif out_dw is not None or out_db is not None:
+        raise ValueError("dense_softmax_ce: out_dw / out_db need want_grad")
+    with _on_device(x):
+        return _dense_softmax_ce(x, w, bias, labels, dx, dw, db, N, V, K, dev, want_grad)
+
+
+def _dense_softmax_ce(x, w, bias, labels, dx, dw, db, N, V, K, dev, want_grad):
+    st = _stream()
+    if N == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+        return torch.zeros((), dtype=torch.float32, device=dev), dx, dw, db, torch.empty(0, dtype=torch.float32, device=dev)
+    Vp = ceil_div(V, 64) * 64
+    rows = torch.empty(N, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    count = torch.empty(1, dtype=torch.float32, device=dev)
+    zt = torch.empty(N, dtype=torch.float32, device=dev)
+    R = N
+    if want_grad and N * Vp * 2 > CE_PIECE_BYTES:
+        R = max(64, CE_PIECE_BYTES // (Vp * 2) // 256 * 256)
+    R = min(R, N)
+    tile = _ce_logits_tile(R, V)
+    nst = _ce_stats_cols(V, tile)
+    stats = torch.empty(R, nst, 2, dtype=torch.float32, device=dev)
+    E = xs = g = g2 = acc_w = acc_b = None
+    if want_grad:
+        E = torch.empty(R, Vp, dtype=torch.bfloat16, device=dev)
+        xs = torch.empty(R, K, dtype=torch.bfloat16, device=dev)
+        g = torch.empty(R, dtype=torch.float32, device=dev)
+        g2 = torch.zeros(2, ceil_div(R, 64) * 64, dtype=torch.bfloat16, device=dev)
+        if R < N:                                   # the row pieces' weight gradients add up in fp32
+            acc_w = dw if dw.dtype == torch.float32 else torch.empty(V, K, dtype=torch.float32, device=dev)
+            if db is not None:
+                acc_b = db if db.dtype == torch.float32 else torch.empty(V, dtype=torch.float32, device=dev)
+        dw_tile = 0 if ceil_div(V, 256) * ceil_div(K, 256) >= 256 else 1
+    for r0 in range(0, N, R):
+        n = min(R, N - r0)
+        xr, lr, rr, zr = x[r0:r0 + n], labels[r0:r0 + n], rows[r0:r0 + n], zt[r0:r0 + n]
+        _rc(_ce_logits(w.data_ptr(), xr.data_ptr(), _p(bias), lr.data_ptr(), n, V, K, Vp, _p(E), stats.data_ptr(),
+                       zr.data_ptr(), labels.data_ptr(), N, count.data_ptr() if r0 == 0 else None, tile, st), "ce_logits")
+        if want_grad and 0 < r0 and n < R:
+            g2.zero_()                              # a shorter last piece: its k padding must read as zero
+        _rc(_ce_rows(stats.data_ptr(), nst, _CE_WAVE_COLS[tile], zr.data_ptr(), lr.data_ptr(), count.data_ptr(), n, V, K,
+                     Vp, _p(E), xr.data_ptr(), _p(xs), rr.data_ptr(), _p(g), _p(g2), g2.shape[1] if want_grad else 0, st),
+            "ce_rows")
+        if not want_grad:
+            continue
+        # input gradient: split over the classes until the chip is full
+        bt = 2 if n <= 32 else (1 if ceil_div(n, 256) * ceil_div(K, 256) < 64 else 0)
+        ba, bb = ((256, 256), (128, 128), (128, 32))[bt]
+        ns, per = _ce_split(V, ceil_div(K, ba) * ceil_div(n, bb), 256 if bt == 0 else 512)
+        slab = torch.empty(ns, n, K, dtype=torch.float32, device=dev) if ns > 1 else None
+        _rc(_ce_dx(w.data_ptr(), E.data_ptr(), n, V, K, Vp, ns, per, g.data_ptr(), dx[r0:r0 + n].data_ptr(), _p(slab), bt,
+                   st), "ce_dx")
+        last = r0 + n >= N
+        ow, ob = (dw, db) if last or acc_w is None else (acc_w, acc_b)
+        _rc(_ce_dw(xs.data_ptr(), E.data_ptr(), n, V, K, Vp, g2.data_ptr(), g2.shape[1], _p(acc_w) if r0 else None,
+                   _p(acc_b) if r0 else None, ow.data_ptr(), _p(ob), int(ow.dtype == torch.bfloat16), dw_tile, st), "ce_dw")
+    _rc(_ce_mean(rows.data_ptr(), count.data_ptr(), N, loss.data_ptr(), st), "ce_mean")
+    _done()
+    return loss, dx, dw, db, rows
+
+
+# ------------------------------------------------------------------------------ 8-bit activation checkpoints
+_pack8 = _sig("ddl_pack8", ci, vp, vp, vp, cl, vp)
+_unpack8 = _sig("ddl_unpack8", ci, vp, vp, vp, cl, vp)
+_act_bwd8 = _sig("ddl_act_bwd8", ci, vp, vp, vp, vp, cl, ci, cf, vp)
+_wgrad8 = _sig("ddl_dense_wgrad8", ci, vp, vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, vp, ci, vp)
+
+
+def _chk_packed(q, name="q"):
+    n = q.codes.numel()
+    if not (q.codes.is_cuda and q.codes.dtype == torch.int8 and q.codes.is_contiguous() and q.scales.device == q.codes.device
+            and q.scales.dtype == torch.uint8 and q.scales.is_contiguous() and q.scales.numel() == ceil_div(n, 32)):
+        raise ValueError(f"{name}: codes must be contiguous int8 and scales uint8, one per 32 codes, on one device")
+    if q.codes.dim() < 1 or q.codes.shape[-1] % 8 or q.codes.data_ptr() % 8:
+        raise ValueError(f"{name}: channel dim must be a multiple of 8 and the codes 8-byte aligned")
+    return n
+
+
+def pack8(x):
+    from .functional import Packed8
+    _chk_act(x, "x")
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(ceil_div(x.numel(), 32), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        with _on_device(x):
+            _rc(_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _stream()), "pack8")
+            _done()
+    return Packed8(codes, scales)
+
+
+def unpack8(q, out=None):
+    n = _chk_packed(q)
+    y = torch.empty(q.codes.shape, dtype=torch.bfloat16, device=q.codes.device) if out is None else out
+    if out is not None:
+        _chk_out(out, n, (torch.bfloat16,), q.codes, "out")
+    if n:
+        with _on_device(y):
+            _rc(_unpack8(q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), n, _stream()), "unpack8")
+            _done()
+    return y
+
+
+def act_bwd8(dy, q, kind, alpha=0.3):
+    if kind in (None, "linear"):
+        return dy
+    _chk_act(dy, "dy")
+    n = _chk_packed(q)
+    if dy.shape != q.codes.shape or dy.device != q.codes.device:
+        raise ValueError(f"act_bwd8: dy {tuple(dy.shape)} on {dy.device}, checkpoint {tuple(q.codes.shape)} on {q.codes.device}")
+    dx = torch.empty_like(dy)
+    if n:
+        with _on_device(dy):
+            _rc(_act_bwd8(dy.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), dx.data_ptr(), n, ACT_CODE[kind], alpha,
+                          _stream()), "act_bwd8")
+            _done()
+    return dx
+
+
+def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
+    """dw [O][Kp] = dy^T x, db [O] = column sums of dy, x [R][Kp] read from its 8-bit checkpoint; fp32."""
+    _chk_act(dy, "dy")
+    _chk_packed(q)
+    x = q.codes
+    if x.dim() != 2 or dy.dim() != 2 or x.shape[0] != dy.shape[0] or x.device != dy.device:
+        raise ValueError(f"dense_wgrad8: checkpoint {tuple(x.shape)} and dy {tuple(dy.shape)} must be [R][K] and [R][O] on one "
+                         "device")
+    R, K = x.shape
+    Op = dy.shape[1]
+    O = Op if n_out is None else int(n_out)
+    if not 0 < O <= Op or K < 8 or max(R, K, Op) >= 1 << 24:
+        raise ValueError(f"dense_wgrad8: R={R} K={K} O={O} of {Op} outside the supported range")
+    dev = dy.device
+    dw = torch.empty(O, K, dtype=torch.float32, device=dev) if out_dw is None else out_dw
+    db = torch.empty(O, dtype=torch.float32, device=dev) if out_db is None else out_db
+    _chk_out(dw, O * K, (torch.float32,), dy, "out_dw")
+    if not (db.device == dev and db.dtype == torch.float32 and db.is_contiguous() and db.numel() == O):
+        raise ValueError(f"out_db: need a contiguous fp32 vector of {O} elements on {dev}")
+    with _on_device(dy):
+        if R == 0:
+            dw.zero_()
+            db.zero_()
+            return dw, db
+        tile = 0 if ceil_div(K, 256) * ceil_div(O, 256) >= 192 else (1 if ceil_div(K, 128) * ceil_div(O, 128) >= 256 else 2)
+        t = (256, 128, 64)[tile]
+        steps = ceil_div(R, 64)
+        ns = max(1, min(512 // (ceil_div(K, t) * ceil_div(O, t)), steps // 4, 64))
+        per = ceil_div(steps, ns) * 64
+        ns = ceil_div(R, per)
+        sw = torch.empty(ns, O, K, dtype=torch.float32, device=dev) if ns > 1 else None
+        sb = torch.empty(ns, O, dtype=torch.float32, device=dev) if ns > 1 else None
+        xh = unpack8(q)
+        _rc(_wgrad8(xh.data_ptr(), dy.data_ptr(), R, K, Op, O, ns, per, dw.data_ptr(), db.data_ptr(), _p(sw), _p(sb), tile,
+                    _stream()), "dense_wgrad8")
+        _done()
+    return dw, db

@@ -1,0 +1,335 @@
+"""dense_softmax_ce against its definition in 64 bits, on the CPU path and on the device.
+
+Bounds.  u = 2^-8 is the largest relative error of a rounding to bf16, 2^-24 to fp32.  With dl the exact gradient of the
+logits and sums of absolute values in 64 bits:
+  rows   the logits carry K fp32 additions, (K + 2) 2^-24 sum |x||w| at the row's largest; it enters the label's logit and
+         the log-sum, hence twice; the exponential, the sum and the logarithm add 2^-20 (1 + |lse| + |z_label|).
+  dx     E (or its label entry) is rounded to bf16 once, the result once: u sum_v |dl||w| + u |dx|, plus the logits' error in
+         p (2 relative terms of it) and V fp32 additions
+  dw     E once, the scaled x once, the result once (bf16 output): (2 u + u^2) sum_r |dl||x| + u |dw|
+  db     E once, the result once: u sum_r |dl| + u |db|"""
+import math
+
+import pytest
+import torch
+
+from distributeddeeplearning_amd.ops import functional as F
+
+U16, U32 = 2.0 ** -8, 2.0 ** -24
+
+
+def make(N, K, V, seed=0, scale=1.0, bias=True, drop=0.0, mask=0.0):
+    g = torch.Generator().manual_seed(seed)
+    Kp = (K + 7) // 8 * 8
+    x, w = torch.zeros(N, Kp), torch.zeros(V, Kp)
+    x[:, :K] = torch.randn(N, K, generator=g) * scale
+    w[:, :K] = torch.randn(V, K, generator=g) * (1.5 / math.sqrt(K))
+    b = torch.randn(V, generator=g) * 0.3 if bias else None
+    labels = torch.randint(0, V, (N,), generator=g)
+    if mask and b is not None:
+        off = torch.rand(V, generator=g) < mask
+        off[labels] = False
+        b[off] = -math.inf
+    if drop:
+        labels[torch.rand(N, generator=g) < drop] = -1
+    return x.bfloat16(), w.bfloat16(), b, labels
+
+
+def exact(x, w, b, labels):
+    """The definition in 64 bits with the sums of absolute values its error bounds need."""
+    live = labels >= 0
+    x, w = torch.where(live[:, None], x.double(), 0.0), w.double()
+    z = x @ w.t() + (0 if b is None else b.double())
+    at = labels.clamp_min(0)[:, None]
+    lse = torch.logsumexp(z, 1)
+    zt = z.gather(1, at)[:, 0]
+    rows = torch.where(live, lse - zt, 0.0)
+    cnt = max(int(live.sum()), 1)
+    dl = torch.exp(z - lse[:, None])
+    dl.scatter_add_(1, at, torch.full_like(at, -1, dtype=torch.float64))
+    dl = torch.where(live[:, None], dl / cnt, 0.0)
+    K, V = x.shape[1], w.shape[0]
+    az = (x.abs() @ w.abs().t()).amax(1) + (0 if b is None else b[torch.isfinite(b)].abs().max().double())
+    ez = (K + 4) * U32 * az                                     # error of a logit
+    p = dl.abs()
+    dp = p * (2 * ez[:, None] + 2.0 ** -20) + (2 * ez[:, None] + 2.0 ** -20) * torch.where(live[:, None], torch.exp(z - lse[:, None]) / cnt, 0.0)
+    return dict(rows=rows, loss=rows.sum() / cnt, dx=dl @ w, dw=dl.t() @ x, db=dl.sum(0),
+                t_rows=2 * ez + 2.0 ** -20 * (1 + lse.abs() + zt.abs()),
+                a_dx=p @ w.abs(), a_dw=p.t() @ x.abs(), a_db=p.sum(0),
+                e_dx=dp @ w.abs(), e_dw=dp.t() @ x.abs(), e_db=dp.sum(0), n=x.shape[0], V=V)
+
+
+def check(out, ref, dtype=torch.float32, x_dtype=torch.bfloat16, device=True):
+    loss, dx, dw, db, rows = out
+    u = U16 if device else 0.0
+    uo = U16 if dtype == torch.bfloat16 else U32
+    ux = U16 if x_dtype == torch.bfloat16 else U32
+    err = (rows.double().cpu() - ref["rows"]).abs()
+    assert (err <= ref["t_rows"]).all(), f"rows off by {err.max():.3g}"
+    assert abs(float(loss) - float(ref["loss"])) <= float(ref["t_rows"].max()) + U32 * abs(float(ref["loss"]))
+    if dx is None:
+        return
+    for name, got, lim in (
+            ("dx", dx, (u + ref["V"] * U32) * ref["a_dx"] + ref["e_dx"] + ux * ref["dx"].abs()),
+            ("dw", dw, (2 * u + u * u + ref["n"] * U32) * ref["a_dw"] + ref["e_dw"] + uo * ref["dw"].abs()),
+            ("db", db, (u + ref["n"] * U32 + 2.0 ** -16) * ref["a_db"] + ref["e_db"] + uo * ref["db"].abs())):
+        if got is None:
+            continue
+        err = (got.double().cpu() - ref[name]).abs()
+        lim = lim * 1.01 + 1e-30                               # second-order terms
+        assert torch.isfinite(got).all(), name
+        assert (err <= lim).all(), f"{name}: {float((err / lim).max()):.3g} of its bound"
+
+
+# ------------------------------------------------------------------------------------------------ CPU path
+@pytest.mark.parametrize("N,K,V", [(1, 8, 1), (3, 5, 70), (17, 30, 333)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_cpu_matches_definition(N, K, V, bias):
+    x, w, b, lab = make(N, K, V, bias=bias, drop=0.2)
+    ref = exact(x, w, b, lab)
+    check(F.dense_softmax_ce(x.float(), w.float(), b, lab), ref, x_dtype=torch.float32, device=False)
+    loss, dx, dw, db, rows = F.dense_softmax_ce(x.float(), w.float(), b, lab, want_grad=False)
+    assert dx is None and dw is None and db is None
+
+
+def test_cpu_gradients_match_differences():
+    x, w, b, lab = make(5, 8, 70, drop=0.3)
+    x, w = x.double(), w.double()
+    _, dx, dw, db, _ = F.dense_softmax_ce(x, w, b, lab)
+
+    def loss(x, w, b):
+        z = x @ w.t() + b
+        live = lab >= 0
+        return -(torch.log_softmax(z, 1).gather(1, lab.clamp_min(0)[:, None])[:, 0][live]).sum() / live.sum()
+    h = 1e-5
+    for t, g, k in ((x, dx, 0), (w, dw, 1), (b.double(), db, 2)):
+        for i in (0, 3, t.numel() - 1):
+            args = [x, w, b.double()]
+            lo, hi = t.clone(), t.clone()
+            lo.view(-1)[i] -= h
+            hi.view(-1)[i] += h
+            args[k] = hi
+            up = loss(*args)
+            args[k] = lo
+            d = (up - loss(*args)) / (2 * h)
+            # central difference: h^2 / 6 times a third derivative below 10, and the fp32 of the CPU path
+            assert abs(float(d) - float(g.reshape(-1)[i])) < 1e-5
+
+
+def test_cpu_rows_without_label_and_bad_labels():
+    x, w, b, lab = make(6, 16, 80)
+    lab[2] = -1
+    lab[4] = -100
+    xn = x.float().clone()
+    xn[2] = math.nan
+    xn[4] = math.inf
+    loss, dx, dw, db, rows = F.dense_softmax_ce(xn, w.float(), b, lab)
+    check((loss, dx, dw, db, rows), exact(x, w, b, lab), x_dtype=torch.float32, device=False)
+    assert (dx[[2, 4]] == 0).all() and (rows[[2, 4]] == 0).all()
+    none = F.dense_softmax_ce(xn, w.float(), b, torch.full((6,), -1))
+    assert float(none[0]) == 0 and all((t == 0).all() for t in none[1:])
+    lab2 = lab.clone()
+    lab2[0] = 80
+    loss, dx, dw, db, rows = F.dense_softmax_ce(x.float(), w.float(), b, lab2)
+    assert math.isnan(float(loss)) and math.isnan(float(rows[0])) and torch.isfinite(rows[1:]).all()
+    assert (dx[0] == 0).all() and torch.isfinite(dw).all()
+
+
+def test_cpu_refusals():
+    x, w, b, lab = make(4, 16, 80)
+    x, w = x.float(), w.float()
+    for bad in (dict(w=w[:, :8]), dict(labels=lab[:3]), dict(labels=lab.int()), dict(bias=b[:79])):
+        a = dict(x=x, w=w, bias=b, labels=lab)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            F.dense_softmax_ce(**a)
+    with pytest.raises(ValueError):
+        F.dense_softmax_ce(x, w, b, lab, want_grad=False, out_dw=torch.empty(80, 16))
+    with pytest.raises(ValueError):
+        F.dense_softmax_ce(x, w, b, lab, out_dw=torch.empty(80, 8))
+    with pytest.raises(ValueError):
+        F.dense_softmax_ce(x, w, None, lab, out_db=torch.empty(80))
+
+
+# ------------------------------------------------------------------------------------------------ device
+def cuda(x, w, b, lab):
+    return x.cuda(), w.cuda(), None if b is None else b.cuda(), lab.cuda()
+
+
+SHAPES = [(1, 8, 1), (1, 16, 65), (2, 24, 1000), (5, 8, 128), (16, 64, 64), (31, 40, 333), (33, 136, 4099), (64, 120, 64),
+          (130, 200, 777), (257, 72, 2051), (300, 520, 515), (513, 264, 769)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_train(N, K, V, dtype):
+    a = make(N, K, V, seed=N + V, drop=0.1 if N > 4 else 0.0)
+    out = F.dense_softmax_ce(*cuda(*a), grad_dtype=dtype)
+    assert out[1].dtype == torch.bfloat16 and out[2].dtype == dtype and out[3].dtype == dtype
+    check(out, exact(*a), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", SHAPES)
+def test_score(N, K, V):
+    a = make(N, K, V, seed=7, drop=0.1 if N > 4 else 0.0)
+    out = F.dense_softmax_ce(*cuda(*a), want_grad=False)
+    assert out[1] is None and out[2] is None and out[3] is None
+    check(out, exact(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
+@pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (260, 136, 600)])
+def test_every_tile(tile, N, K, V, monkeypatch):
+    from distributeddeeplearning_amd.ops import hip
+    monkeypatch.setattr(hip, "_ce_logits_tile", lambda n, v: tile)
+    a = make(N, K, V, seed=tile, drop=0.1)
+    check(F.dense_softmax_ce(*cuda(*a)), exact(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias,mask", [(False, 0.0), (True, 0.5), (True, 0.97)])
+def test_bias_and_classes_switched_off(bias, mask):
+    a = make(70, 40, 900, seed=3, bias=bias, mask=mask)
+    out = F.dense_softmax_ce(*cuda(*a))
+    assert (out[3] is None) == (not bias)
+    check(out, exact(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [-3000.0, -100.0, 60.0, 300.0, 3000.0])
+@pytest.mark.parametrize("part", [False, True])
+def test_logits_far_from_zero(shift, part):
+    """References other than 0: all classes far away, or one stretch of them (tiles of one row disagree)."""
+    x, w, b, lab = make(40, 64, 1500, seed=5)
+    if part:
+        b[300:700] += shift
+        lab[lab % 3 == 0] = 500
+    else:
+        b += shift
+    a = (x, w, b, lab)
+    check(F.dense_softmax_ce(*cuda(*a)), exact(*a))
+
+
+@pytest.mark.gpu
+def test_large_logits_saturate():
+    a = make(64, 64, 700, seed=6, scale=40.0)
+    check(F.dense_softmax_ce(*cuda(*a)), exact(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [2, 40, 300])
+def test_rows_without_label_hold_anything(N):
+    x, w, b, lab = make(N, 48, 520, seed=8)
+    lab[1::2] = -1
+    xb = x.clone()
+    xb[1::4], xb[3::4] = math.nan, math.inf
+    out = F.dense_softmax_ce(*cuda(xb, w, b, lab))
+    check(out, exact(x, w, b, lab))
+    assert (out[1][1::2] == 0).all() and (out[4][1::2] == 0).all()
+    none = F.dense_softmax_ce(*cuda(xb, w, b, torch.full((N,), -1)))
+    assert float(none[0]) == 0 and all((t == 0).all() for t in none[1:])
+
+
+@pytest.mark.gpu
+def test_bad_label_nan_row_and_no_class_left():
+    x, w, b, lab = make(9, 16, 300, seed=9)
+    lab2 = lab.clone()
+    lab2[4] = 300
+    loss, dx, dw, db, rows = F.dense_softmax_ce(*cuda(x, w, b, lab2))
+    assert math.isnan(float(loss)) and math.isnan(float(rows[4])) and int(torch.isnan(rows).sum()) == 1
+    assert (dx[4] == 0).all() and torch.isfinite(dw).all() and torch.isfinite(db).all()
+    xn = x.clone()
+    xn[2, 3] = math.nan
+    loss, dx, dw, db, rows = F.dense_softmax_ce(*cuda(xn, w, b, lab))
+    assert math.isnan(float(rows[2])) and int(torch.isnan(rows).sum()) == 1 and torch.isnan(dx[2]).all()
+    assert torch.isfinite(dx[:2]).all() and torch.isfinite(dx[3:]).all() and torch.isnan(dw).all()
+    off = torch.full_like(b, -math.inf)
+    loss, dx, dw, db, rows = F.dense_softmax_ce(*cuda(x, w, off, lab))
+    assert torch.isnan(rows).all() and torch.isnan(dx).all()
+    b2 = b.clone()                                            # the label's own class switched off: loss inf, gradient exists
+    b2[lab[0]] = -math.inf
+    loss, dx, dw, db, rows = F.dense_softmax_ce(*cuda(x[:1], w, b2, lab[:1]))
+    assert float(rows[0]) == math.inf
+    p = torch.softmax(x[:1].double() @ w.double().t() + b2.double(), 1)
+    p[0, lab[0]] -= 1
+    lim = U16 * (p.abs() @ w.double().abs()) + U16 * (p @ w.double()).abs() + 1e-5
+    assert ((dx.double().cpu() - p @ w.double()).abs() <= lim).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [512, 600, 777])
+def test_row_pieces(N, dtype, monkeypatch):
+    from distributeddeeplearning_amd.ops import hip
+    a = make(N, 72, 700, seed=N, drop=0.1)
+    d = cuda(*a)
+    monkeypatch.setattr(hip, "CE_PIECE_BYTES", 256 * 704 * 2)
+    out = F.dense_softmax_ce(*d, grad_dtype=dtype)
+    check(out, exact(*a), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_out_tensors_and_empty_batch(dtype):
+    a = make(20, 40, 130, seed=2)
+    d = cuda(*a)
+    flat = torch.full((130 * 40 + 136,), 7.0, dtype=dtype, device="cuda")
+    dw, db = flat[:130 * 40].view(130, 40), flat[130 * 40:130 * 40 + 130]
+    out = F.dense_softmax_ce(*d, out_dw=dw, out_db=db)
+    assert out[2] is dw and out[3] is db and (flat[-6:] == 7).all()
+    check(out, exact(*a), dtype)
+    out = F.dense_softmax_ce(d[0][:0], d[1], d[2], d[3][:0], out_dw=dw, out_db=db)
+    assert float(out[0]) == 0 and (dw == 0).all() and (db == 0).all() and out[4].numel() == 0 and (flat[-6:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_same_bits_twice_and_on_another_stream():
+    a = make(150, 200, 3001, seed=4)
+    d = cuda(*a)
+    one = F.dense_softmax_ce(*d)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        two = F.dense_softmax_ce(*d)
+    torch.cuda.current_stream().wait_stream(s)
+    for p, q in zip(one, two):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed():
+    from distributeddeeplearning_amd.utils import hipgraph
+    a = make(100, 64, 900, seed=1, drop=0.1)
+    d = cuda(*a)
+    x, lab = d[0].clone(), d[3].clone()
+    F.dense_softmax_ce(x, d[1], d[2], lab)
+    hipgraph.quiesce()
+    g, out = hipgraph.capture(lambda: F.dense_softmax_ce(x, d[1], d[2], lab))
+    for seed in (11, 12, 13):
+        b = make(100, 64, 900, seed=seed, drop=0.1)
+        x.copy_(b[0])
+        lab.copy_(b[3])
+        g.replay()
+        torch.cuda.synchronize()
+        want = F.dense_softmax_ce(x, d[1], d[2], lab)
+        for p, q in zip(out, want):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_refusals():
+    x, w, b, lab = cuda(*make(8, 16, 80))
+    ok = dict(x=x, w=w, bias=b, labels=lab)
+    wide = torch.zeros(8, 32, dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(w=w[:, :8]), dict(w=w.float()), dict(x=wide[:, ::2]), dict(x=x[:, :15].contiguous()), dict(x=x[0]),
+                dict(labels=lab[:7]), dict(labels=lab.int()), dict(labels=lab.cpu()), dict(bias=b[:79].contiguous()),
+                dict(bias=b.double()), dict(bias=b.cpu()), dict(out_dw=torch.empty(80, 8, device="cuda")),
+                dict(out_dw=torch.empty(80, 16, device="cuda", dtype=torch.float16)), dict(grad_dtype=torch.float16),
+                dict(out_db=torch.empty(79, device="cuda")), dict(want_grad=False, out_dw=torch.empty(80, 16, device="cuda")),
+                dict(out_dw=torch.empty(80, 16, device="cuda"), out_db=torch.empty(80, device="cuda", dtype=torch.bfloat16)),
+                dict(bias=None, out_db=torch.empty(80, device="cuda")), dict(out_dw=torch.empty(80, 16))):
+        with pytest.raises(ValueError):
+            F.dense_softmax_ce(**{**ok, **bad})
