@@ -2402,17 +2402,14 @@ def conv_wgrad(x, dy, g: ConvGeom, layout="A", out=None, box=None, x_affine=None
 
 
 # ------------------------------------------------------------------------------ wide softmax head
-_ce_stats_cols = _sig("ddl_ce_stats_cols", ci, ci, ci)
-_ce_logits = _sig("ddl_ce_logits", ci, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, ci, vp, ci, vp)
-_ce_rows = _sig("ddl_ce_rows", ci, vp, ci, ci, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, vp, vp, ci, vp)
-_ce_mean = _sig("ddl_ce_mean", ci, vp, vp, ci, vp, vp)
-_ce_dx = _sig("ddl_ce_dx", ci, vp, vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, ci, vp)
-_ce_dw = _sig("ddl_ce_dw", ci, vp, vp, ci, ci, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, vp)
+_dense_ce_ws = _sig("ddl_dense_ce_workspace", cl, ci, ci, ci, ci, ci, cl, ci)
+_dense_ce = _sig("ddl_dense_ce", ci, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, ci, vp, cl, cl, ci, vp)
 
-# Workspace of a training call in bytes: the exponentials of one piece of rows, 2 bytes per row and class.  4 GiB is
-# 8192 rows of 262144 classes and 1.4 % of the card's memory; a piece costs one more pass over the fp32 weight gradient.
+# Bound on the exponentials a training call keeps at a time, 2 bytes per row and class; a batch that needs more goes
+# through in pieces of rows (at most 8192), each of which reads and writes the fp32 weight gradient once more.  4 GiB,
+# 1.4 % of the card's memory, is 8192 rows of 262144 classes.
 CE_PIECE_BYTES = int(os.environ.get("DDL_CE_PIECE_BYTES", str(4 << 30)))
-_CE_WAVE_COLS = {0: 128, 1: 64, 2: 32, 3: 16}
+CE_TILE = -1                # tile of the logits product: -1 = by the sizes (csrc/hip/dense_ce.hip ce_plan)
 
 
 def _rc(rc, what):
@@ -2433,25 +2430,8 @@ def _chk_out(t, n, dtypes, like, name):
         raise ValueError(f"{name}: not 16-byte aligned")
 
 
-def _ce_logits_tile(n, V):
-    """Rows x classes of a tile: as few padding rows as the batch leaves, and enough blocks for 256 CUs."""
-    if n <= 32:
-        return 3 if V < 256 * 128 else 2
-    if n <= 128 or ceil_div(V, 256) * ceil_div(n, 256) < 256:
-        return 1
-    return 0
-
-
 def ceil_div(a, b):
     return -(-a // b)
-
-
-def _ce_split(V, tiles, want):
-    """(splits, classes per split): the reduction over the classes is cut until `want` blocks run."""
-    steps = ceil_div(V, 64)
-    ns = max(1, min(want // max(tiles, 1), steps // 4, 64))
-    per = ceil_div(steps, ns) * 64
-    return ceil_div(V, per), per
 
 
 def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):
@@ -2464,7 +2444,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
     N, K = x.shape
     V = w.shape[0]
     dev = x.device
-    if V < 1 or K < 8 or max(N, V) >= 1 << 28 or K >= 1 << 22:
+    if V < 1 or K < 8 or N >= 1 << 28 or max(V, K) >= (1 << 22) - 64:
         raise ValueError(f"dense_softmax_ce: N={N} K={K} V={V} outside the supported range")
     for t, name in ((w, "w"), (bias, "bias"), (labels, "labels"), (out_dw, "out_dw"), (out_db, "out_db")):
         if t is not None and t.device != dev:
@@ -2494,64 +2474,22 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
     elif out_dw is not None or out_db is not None:
         raise ValueError("dense_softmax_ce: out_dw / out_db need want_grad")
     with _on_device(x):
-        return _dense_softmax_ce(x, w, bias, labels, dx, dw, db, N, V, K, dev, want_grad)
-
-
-def _dense_softmax_ce(x, w, bias, labels, dx, dw, db, N, V, K, dev, want_grad):
-    st = _stream()
-    if N == 0:
-        for t in (dw, db):
-            if t is not None:
-                t.zero_()
-        return torch.zeros((), dtype=torch.float32, device=dev), dx, dw, db, torch.empty(0, dtype=torch.float32, device=dev)
-    Vp = ceil_div(V, 64) * 64
-    rows = torch.empty(N, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    count = torch.empty(1, dtype=torch.float32, device=dev)
-    zt = torch.empty(N, dtype=torch.float32, device=dev)
-    R = N
-    if want_grad and N * Vp * 2 > CE_PIECE_BYTES:
-        R = max(64, CE_PIECE_BYTES // (Vp * 2) // 256 * 256)
-    R = min(R, N)
-    tile = _ce_logits_tile(R, V)
-    nst = _ce_stats_cols(V, tile)
-    stats = torch.empty(R, nst, 2, dtype=torch.float32, device=dev)
-    E = xs = g = g2 = acc_w = acc_b = None
-    if want_grad:
-        E = torch.empty(R, Vp, dtype=torch.bfloat16, device=dev)
-        xs = torch.empty(R, K, dtype=torch.bfloat16, device=dev)
-        g = torch.empty(R, dtype=torch.float32, device=dev)
-        g2 = torch.zeros(2, ceil_div(R, 64) * 64, dtype=torch.bfloat16, device=dev)
-        if R < N:                                   # the row pieces' weight gradients add up in fp32
-            acc_w = dw if dw.dtype == torch.float32 else torch.empty(V, K, dtype=torch.float32, device=dev)
-            if db is not None:
-                acc_b = db if db.dtype == torch.float32 else torch.empty(V, dtype=torch.float32, device=dev)
-        dw_tile = 0 if ceil_div(V, 256) * ceil_div(K, 256) >= 256 else 1
-    for r0 in range(0, N, R):
-        n = min(R, N - r0)
-        xr, lr, rr, zr = x[r0:r0 + n], labels[r0:r0 + n], rows[r0:r0 + n], zt[r0:r0 + n]
-        _rc(_ce_logits(w.data_ptr(), xr.data_ptr(), _p(bias), lr.data_ptr(), n, V, K, Vp, _p(E), stats.data_ptr(),
-                       zr.data_ptr(), labels.data_ptr(), N, count.data_ptr() if r0 == 0 else None, tile, st), "ce_logits")
-        if want_grad and 0 < r0 and n < R:
-            g2.zero_()                              # a shorter last piece: its k padding must read as zero
-        _rc(_ce_rows(stats.data_ptr(), nst, _CE_WAVE_COLS[tile], zr.data_ptr(), lr.data_ptr(), count.data_ptr(), n, V, K,
-                     Vp, _p(E), xr.data_ptr(), _p(xs), rr.data_ptr(), _p(g), _p(g2), g2.shape[1] if want_grad else 0, st),
-            "ce_rows")
-        if not want_grad:
-            continue
-        # input gradient: split over the classes until the chip is full
-        bt = 2 if n <= 32 else (1 if ceil_div(n, 256) * ceil_div(K, 256) < 64 else 0)
-        ba, bb = ((256, 256), (128, 128), (128, 32))[bt]
-        ns, per = _ce_split(V, ceil_div(K, ba) * ceil_div(n, bb), 256 if bt == 0 else 512)
-        slab = torch.empty(ns, n, K, dtype=torch.float32, device=dev) if ns > 1 else None
-        _rc(_ce_dx(w.data_ptr(), E.data_ptr(), n, V, K, Vp, ns, per, g.data_ptr(), dx[r0:r0 + n].data_ptr(), _p(slab), bt,
-                   st), "ce_dx")
-        last = r0 + n >= N
-        ow, ob = (dw, db) if last or acc_w is None else (acc_w, acc_b)
-        _rc(_ce_dw(xs.data_ptr(), E.data_ptr(), n, V, K, Vp, g2.data_ptr(), g2.shape[1], _p(acc_w) if r0 else None,
-                   _p(acc_b) if r0 else None, ow.data_ptr(), _p(ob), int(ow.dtype == torch.bfloat16), dw_tile, st), "ce_dw")
-    _rc(_ce_mean(rows.data_ptr(), count.data_ptr(), N, loss.data_ptr(), st), "ce_mean")
-    _done()
+        if N == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+            return torch.zeros((), dtype=torch.float32, device=dev), dx, dw, db, torch.empty(0, dtype=torch.float32, device=dev)
+        out = torch.empty(N + 1, dtype=torch.float32, device=dev)
+        loss, rows = out[N], out[:N]
+        bf = int(want_grad and dw.dtype == torch.bfloat16)
+        nws = _dense_ce_ws(N, V, K, int(want_grad), bf, CE_PIECE_BYTES, CE_TILE)
+        if nws < 0:
+            raise ValueError(f"dense_softmax_ce: N={N} K={K} V={V} outside the kernels' range")
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        _rc(_dense_ce(x.data_ptr(), w.data_ptr(), _p(bias), labels.data_ptr(), N, V, K, loss.data_ptr(), rows.data_ptr(),
+                      _p(dx), _p(dw), _p(db), bf, ws.data_ptr(), nws, CE_PIECE_BYTES, CE_TILE, _stream()),
+            "dense_softmax_ce")
+        _done()
     return loss, dx, dw, db, rows
 
 

@@ -4,8 +4,8 @@ Bounds.  u = 2^-8 is the largest relative error of a rounding to bf16, 2^-24 to 
 logits and sums of absolute values in 64 bits:
   rows   the logits carry K fp32 additions, (K + 2) 2^-24 sum |x||w| at the row's largest; it enters the label's logit and
          the log-sum, hence twice; the exponential, the sum and the logarithm add 2^-20 (1 + |lse| + |z_label|).
-  dx     E (or its label entry) is rounded to bf16 once, the result once: u sum_v |dl||w| + u |dx|, plus the logits' error in
-         p (2 relative terms of it) and V fp32 additions
+  dx     E is rounded to bf16 once, the result once: u sum_v |dl||w| + u |dx|, plus the logits' error in p (2 relative terms
+         of it) and V fp32 additions
   dw     E once, the scaled x once, the result once (bf16 output): (2 u + u^2) sum_r |dl||x| + u |dw|
   db     E once, the result once: u sum_r |dl| + u |db|"""
 import math
@@ -184,7 +184,7 @@ def test_score(N, K, V):
 @pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (260, 136, 600)])
 def test_every_tile(tile, N, K, V, monkeypatch):
     from distributeddeeplearning_amd.ops import hip
-    monkeypatch.setattr(hip, "_ce_logits_tile", lambda n, v: tile)
+    monkeypatch.setattr(hip, "CE_TILE", tile)
     a = make(N, K, V, seed=tile, drop=0.1)
     check(F.dense_softmax_ce(*cuda(*a)), exact(*a))
 
@@ -283,6 +283,28 @@ def test_out_tensors_and_empty_batch(dtype):
     check(out, exact(*a), dtype)
     out = F.dense_softmax_ce(d[0][:0], d[1], d[2], d[3][:0], out_dw=dw, out_db=db)
     assert float(out[0]) == 0 and (dw == 0).all() and (db == 0).all() and out[4].numel() == 0 and (flat[-6:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V,classes", [(200, 500, 1), (700, 300, 3), (1500, 4000, 40)])
+def test_many_rows_of_one_class_and_label_terms(N, V, classes):
+    """Labels repeat; the label terms are exact, so a class that only its own rows' label terms reach (p ~ 0 elsewhere) has
+    its dw row to the output's rounding."""
+    x, w, b, lab = make(N, 64, V, seed=N, drop=0.05)
+    lab = torch.where(lab >= 0, lab % classes * 7, lab)
+    a = (x, w, b, lab)
+    ref = exact(*a)
+    out = F.dense_softmax_ce(*cuda(*a))
+    check(out, ref)
+    # the label entries carry no bf16 rounding: what is left is u times the other entries of each sum
+    live = lab >= 0
+    oh = torch.zeros(N, V, dtype=torch.float64)
+    oh[live.nonzero()[:, 0], lab[live]] = 1.0
+    xd = torch.where(live[:, None], x.double(), 0.0)
+    z = xd @ w.double().t() + b.double()
+    other = torch.softmax(z, 1) * (1 - oh) * live[:, None] / int(live.sum())
+    lim = (2 * U16 + U16 ** 2) * (other.t() @ xd.abs()) + N * U32 * ref["a_dw"] + ref["e_dw"] + 2 * U32 * ref["a_dw"]
+    assert ((out[2].double().cpu() - ref["dw"]).abs() <= 1.01 * lim + 1e-30).all()
 
 
 @pytest.mark.gpu
