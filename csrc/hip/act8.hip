@@ -156,16 +156,16 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void dens
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
     const bool do_db = ta == 0 && wa == 0 && a.db;
-    f32x4 acc[T::NA][T::NB], bacc[T::NB];
-#pragma unroll
-    for (int j = 0; j < T::NB; ++j) bacc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const short one = fr == 0 ? 0x3f80 : 0;                  // db: one more product per fragment against a row of ones
-    const s16x8 ones = {one, one, one, one, one, one, one, one};
+    f32x4 acc[T::NA][T::NB], bacc = {0.f, 0.f, 0.f, 0.f};
+    static_assert(T::NB <= 4, "rows of the bias accumulator");
     T::run(a.x, a.dy, k0, o0, r0, r1, smem, acc, [&](int, const bf16x8_t (&bv)[T::NB]) {
-        if (do_db) {
+        if (do_db) {                 // db: one more product per fragment j, against a fragment whose row 4 j is ones
 #pragma unroll
-            for (int j = 0; j < T::NB; ++j)
-                bacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), bv[j], bacc[j], 0, 0, 0);
+            for (int j = 0; j < T::NB; ++j) {
+                const short one = fr == 4 * j ? 0x3f80 : 0;
+                const s16x8 ones = {one, one, one, one, one, one, one, one};
+                bacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), bv[j], bacc, 0, 0, 0);
+            }
         }
     });
     float* dw = a.dw + (long)blockIdx.y * a.O * a.K;
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void dens
     for (int j = 0; j < T::NB; ++j) {
         const int o = wo + 16 * j;
         if (o >= a.O) continue;
-        if (do_db && fq == 0) db[o] = bacc[j][0];
+        if (do_db && fq == j) db[o] = bacc[0];
 #pragma unroll
         for (int i = 0; i < T::NA; ++i) {
             const int k = wk + 16 * i;

@@ -481,17 +481,19 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
     const bool do_db = ta == 0 && wa == 0;                     // wave-uniform
-    f32x4 acc[T::NA][T::NB], bacc[T::NB];
-#pragma unroll
-    for (int j = 0; j < T::NB; ++j) bacc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    // db = E^T g: one more matrix instruction per B fragment against a fragment whose rows 0 and 1 are g's two terms
+    f32x4 acc[T::NA][T::NB], bacc = {0.f, 0.f, 0.f, 0.f};
+    static_assert(T::NB <= 4, "rows of the bias accumulator");
+    // db = E^T g: one more matrix instruction per B fragment j, against a fragment whose rows 4 j and 4 j + 1 are g's two
+    // terms and all others zero: one accumulator holds all of them
     T::run(a.xs, a.e, k0, v0, 0, a.N, smem, acc, [&](int k, const bf16x8_t (&bv)[T::NB]) {
         if (do_db) {
             const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + k + 8 * fq);
             const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            const bf16x8_t ga = __builtin_bit_cast(bf16x8_t, fr < 2 ? gv : z);
 #pragma unroll
-            for (int j = 0; j < T::NB; ++j) bacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ga, bv[j], bacc[j], 0, 0, 0);
+            for (int j = 0; j < T::NB; ++j) {
+                const bf16x8_t ga = __builtin_bit_cast(bf16x8_t, (fr & ~1) == 4 * j ? gv : z);
+                bacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ga, bv[j], bacc, 0, 0, 0);
+            }
         }
     });
     const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
@@ -500,8 +502,8 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
         const int v = wv + 16 * j;
         if (v >= a.V) continue;
         const int sl = a.slot[v];
-        if (do_db && fq == 0 && a.db) {
-            float b = bacc[j][0] + bacc[j][1];
+        if (do_db && fq == j && a.db) {
+            float b = bacc[0] + bacc[1];
             if (sl >= 0) b += a.Lb[sl];
             if (a.acc_b) b += a.acc_b[v];
             if (a.out_bf16) ((bf16_t*)a.db)[v] = f2bf(b);
@@ -542,6 +544,7 @@ struct CePlan {
 
 static int ce_cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
+// force_tile: -1, or decimal digits (dw, dx, logits) of the tiles to take, 9 = by the sizes
 static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, int force_tile) {
     CePlan p;
     p.Vp = ce_cdiv(V, 64) * 64;
@@ -554,11 +557,12 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     }
     // as few padding rows as the batch leaves, and enough blocks for 256 CUs
     p.lt = p.R <= 32 ? (V < 256 * 128 ? 3 : 2) : (p.R <= 128 || (long)ce_cdiv(V, 256) * ce_cdiv(p.R, 256) < 256 ? 1 : 0);
-    if (force_tile >= 0) p.lt = force_tile;
+    if (force_tile >= 0 && force_tile % 10 < 4) p.lt = force_tile % 10;
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
     p.wave_cols = cols[p.lt];
-    p.nst = ce_cdiv(V, ba[p.lt]) * (ba[p.lt] / p.wave_cols);
+    p.nst = ce_cdiv(p.Vp, ba[p.lt]) * (ba[p.lt] / p.wave_cols);      // the tiles cover E's zero columns too
     p.xt = p.R <= 32 ? 2 : ((long)ce_cdiv(p.R, 256) * ce_cdiv(K, 256) < 64 ? 1 : 0);
+    if (force_tile >= 0 && force_tile / 10 % 10 < 3) p.xt = force_tile / 10 % 10;
     {
         static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32};
         const long tiles = (long)ce_cdiv(K, xa[p.xt]) * ce_cdiv(p.R, xb[p.xt]);
@@ -571,6 +575,7 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         p.ns = ce_cdiv(V, p.per);
     }
     p.wt = (long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1;
+    if (force_tile >= 0 && force_tile / 100 % 10 < 2) p.wt = force_tile / 100 % 10;
     p.g2_pitch = ce_cdiv(p.R, 64) * 64;
     long o = 0;
     auto take = [&](long bytes) { const long at = o; o += (bytes + 255) / 256 * 256; return at; };
@@ -594,7 +599,7 @@ static int launch_logits(CeLogitsArgs& a, hipStream_t s) {
     if (a.order && 4L * a.N > (long)lds) lds = 4L * a.N;
     constexpr auto kern = ce_logits_kernel<BA, BB, WA, WB, STAGES, STORE>;
     if (int rc = gt_lds<kern>(lds)) return rc;
-    a.map = gt_make_map((a.V + BA - 1) / BA, (a.N + BB - 1) / BB, 8);
+    a.map = gt_make_map((a.Vp + BA - 1) / BA, (a.N + BB - 1) / BB, 8);
     a.nrank = a.order ? (ce_cdiv(a.N, CE_RANK_ROWS) + 7) / 8 * 8 : 8;
     kern<<<a.nrank + gt_grid(a.map), T::NTHR, lds, s>>>(a);
     return gt_launched();
@@ -638,7 +643,7 @@ static bool ce_range_ok(int N, int V, int K) {
 
 // Workspace of one call in bytes (negative: sizes outside the kernels' range)
 DDL_API long ddl_dense_ce_workspace(int N, int V, int K, int train, int out_bf16, long budget, int force_tile) {
-    if (!ce_range_ok(N, V, K) || force_tile > 3) return -1;
+    if (!ce_range_ok(N, V, K) || force_tile > 999) return -1;
     return ce_plan(N, V, K, train, out_bf16, budget, force_tile).bytes;
 }
 
@@ -646,7 +651,7 @@ DDL_API long ddl_dense_ce_workspace(int N, int V, int K, int train, int out_bf16
 DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, const long* labels, int N, int V, int K,
                          float* loss, float* rows, void* dx, void* dw, void* db, int out_bf16, void* ws_, long ws_bytes,
                          long budget, int force_tile, hipStream_t s) {
-    if (!ce_range_ok(N, V, K) || force_tile > 3) return -1;
+    if (!ce_range_ok(N, V, K) || force_tile > 999) return -1;
     const bool train = dx != nullptr;
     const CePlan p = ce_plan(N, V, K, train, out_bf16, budget, force_tile);
     if (ws_bytes < p.bytes || (train && !dw)) return -3;

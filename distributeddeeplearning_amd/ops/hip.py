@@ -2409,7 +2409,7 @@ _dense_ce = _sig("ddl_dense_ce", ci, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp,
 # through in pieces of rows (at most 8192), each of which reads and writes the fp32 weight gradient once more.  4 GiB,
 # 1.4 % of the card's memory, is 8192 rows of 262144 classes.
 CE_PIECE_BYTES = int(os.environ.get("DDL_CE_PIECE_BYTES", str(4 << 30)))
-CE_TILE = -1                # tile of the logits product: -1 = by the sizes (csrc/hip/dense_ce.hip ce_plan)
+CE_TILE = -1                # tiles of the products: -1 = by the sizes, else digits dw, dx, logits (csrc/hip/dense_ce.hip)
 
 
 def _rc(rc, what):
@@ -2577,7 +2577,7 @@ def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
         tile = 0 if ceil_div(K, 256) * ceil_div(O, 256) >= 192 else (1 if ceil_div(K, 128) * ceil_div(O, 128) >= 256 else 2)
         t = (256, 128, 64)[tile]
         steps = ceil_div(R, 64)
-        ns = max(1, min(512 // (ceil_div(K, t) * ceil_div(O, t)), steps // 4, 64))
+        ns = max(1, min((256 if tile == 0 else 512) // (ceil_div(K, t) * ceil_div(O, t)), steps // 4, 64))
         per = ceil_div(steps, ns) * 64
         ns = ceil_div(R, per)
         sw = torch.empty(ns, O, K, dtype=torch.float32, device=dev) if ns > 1 else None

@@ -180,7 +180,7 @@ def test_score(N, K, V):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile", [0, 1, 2, 3])
+@pytest.mark.parametrize("tile", [0, 1, 2, 3, 109, 119, 129, 9, 19, 29])
 @pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (260, 136, 600)])
 def test_every_tile(tile, N, K, V, monkeypatch):
     from distributeddeeplearning_amd.ops import hip
@@ -355,3 +355,15 @@ def test_refusals():
                 dict(bias=None, out_db=torch.empty(80, device="cuda")), dict(out_dw=torch.empty(80, 16))):
         with pytest.raises(ValueError):
             F.dense_softmax_ce(**{**ok, **bad})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", [(3, 24, 65), (20, 40, 97), (31, 72, 1030), (40, 64, 130)])
+def test_padding_classes_are_zero_in_a_dirty_workspace(N, K, V):
+    """The exponentials' columns behind the last class enter the products: they have to be written, not found zero."""
+    a = make(N, K, V, seed=V)
+    d = cuda(*a)
+    for _ in range(3):
+        dirty = [torch.full((1 << s,), 255, dtype=torch.uint8, device="cuda") for s in (14, 16, 18, 20, 20, 21, 22)]
+        del dirty                                              # NaN bits in the allocator's free blocks
+        check(F.dense_softmax_ce(*d), exact(*a))
