@@ -147,12 +147,12 @@ struct Wg8Args {
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void dense_wgrad8_kernel(const Wg8Args a) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int ta, tb;
-    if (!gt_map(a.map, blockIdx.x, ta, tb)) return;
+    int ta, tb, split;
+    if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
     const int k0 = ta * BA, o0 = tb * BB;
-    const int r0 = blockIdx.y * a.per_split, r1 = min(r0 + a.per_split, a.R);
+    const int r0 = split * a.per_split, r1 = min(r0 + a.per_split, a.R);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
     const bool do_db = ta == 0 && wa == 0 && a.db;
@@ -168,8 +168,8 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void dens
             }
         }
     });
-    float* dw = a.dw + (long)blockIdx.y * a.O * a.K;
-    float* db = a.db ? a.db + (long)blockIdx.y * a.O : nullptr;
+    float* dw = a.dw + (long)split * a.O * a.K;
+    float* db = a.db ? a.db + (long)split * a.O : nullptr;
     const int wk = k0 + wa * (BA / WA) + 4 * fq, wo = o0 + wb * (BB / WB) + fr;
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
@@ -234,11 +234,11 @@ DDL_API int ddl_act_bwd8(const void* dy, const void* codes, const void* scales, 
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 static int launch_wgrad8(Wg8Args& a, hipStream_t s) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
     constexpr auto kern = dense_wgrad8_kernel<BA, BB, WA, WB, STAGES>;
     if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
-    a.map = gt_make_map((a.K + BA - 1) / BA, (a.O + BB - 1) / BB, 4);
-    kern<<<dim3(gt_grid(a.map), a.nsplit), T::NTHR, T::LDS_BYTES, s>>>(a);
+    a.map = gt_make_map((a.K + BA - 1) / BA, (a.O + BB - 1) / BB, a.nsplit, 4);
+    kern<<<gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
     return gt_launched();
 }
 

@@ -93,15 +93,15 @@ __device__ __forceinline__ void ce_rank(const CeLogitsArgs& a, char* smem, int b
 
 template <int BA, int BB, int WA, int WB, int STAGES, bool STORE>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_logits_kernel(const CeLogitsArgs a) {
-    using T = GtTile<BA, BB, WA, WB, false, false, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, false, false, STAGES, GT_PLAIN>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x < a.nrank) {
         ce_rank<T::NTHR>(a, smem, blockIdx.x);
         return;
     }
-    int ta, tb;
-    if (!gt_map(a.map, blockIdx.x - a.nrank, ta, tb)) return;
+    int ta, tb, one;
+    if (!gt_map(a.map, blockIdx.x - a.nrank, ta, tb, one)) return;
     const int v0 = ta * BA, r0 = tb * BB;
     if (STORE && tb == 0)
         for (int i = tid; i < BA; i += T::NTHR)
@@ -407,12 +407,12 @@ __device__ __forceinline__ void ce_dx_store(const CeRow& c, const bf16_t* w, int
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dx_kernel(const CeDxArgs a) {
-    using T = GtTile<BA, BB, WA, WB, true, false, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, false, STAGES, GT_FENCE>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int ta, tb;
-    if (!gt_map(a.map, blockIdx.x, ta, tb)) return;
+    int ta, tb, split;
+    if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
     const int k0 = ta * BA, r0 = tb * BB;
-    const int v0 = blockIdx.y * a.per_split, v1 = min(v0 + a.per_split, a.V);
+    const int v0 = split * a.per_split, v1 = min(v0 + a.per_split, a.V);
     f32x4 acc[T::NA][T::NB];
     T::run(a.w, a.e, k0, r0, v0, v1, smem, acc, [](int, const bf16x8_t (&)[T::NB]) {});
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
             if (k >= a.K) continue;
             const f32x4 d = acc[i][j];
             if (a.slab) {
-                *(float4*)(a.slab + ((long)blockIdx.y * a.N + r) * a.K + k) = make_float4(d[0], d[1], d[2], d[3]);
+                *(float4*)(a.slab + ((long)split * a.N + r) * a.K + k) = make_float4(d[0], d[1], d[2], d[3]);
             } else {
                 ce_dx_store(c, a.w.p, a.K, k, d, a.dx + (long)r * a.K + k);
             }
@@ -473,16 +473,22 @@ struct CeDwArgs {
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dw_kernel(const CeDwArgs a) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int ta, tb;
-    if (!gt_map(a.map, blockIdx.x, ta, tb)) return;
+    int ta, tb, one;
+    if (!gt_map(a.map, blockIdx.x, ta, tb, one)) return;
     const int k0 = ta * BA, v0 = tb * BB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
     const bool do_db = ta == 0 && wa == 0;                     // wave-uniform
     f32x4 acc[T::NA][T::NB], bacc = {0.f, 0.f, 0.f, 0.f};
     static_assert(T::NB <= 4, "rows of the bias accumulator");
+    int slots[T::NB];                                          // fetched here: their latency is the loop's
+#pragma unroll
+    for (int j = 0; j < T::NB; ++j) {
+        const int v = v0 + wb * (BB / WB) + 16 * j + fr;
+        slots[j] = v < a.V ? a.slot[v] : -1;
+    }
     // db = E^T g: one more matrix instruction per B fragment j, against a fragment whose rows 4 j and 4 j + 1 are g's two
     // terms and all others zero: one accumulator holds all of them
     T::run(a.xs, a.e, k0, v0, 0, a.N, smem, acc, [&](int k, const bf16x8_t (&bv)[T::NB]) {
@@ -497,11 +503,15 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
         }
     });
     const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
+    // bf16 rows leave through the wave's own LDS patch as whole 16-byte groups (8-byte stores of 16 rows at a time: the
+    // batch-32 case, which is little else than this store, 17 -> 10 us)
+    constexpr int PITCH = BA / WA * 2 + 16;
+    char* patch = smem + wave * (BB / WB) * PITCH;
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int v = wv + 16 * j;
         if (v >= a.V) continue;
-        const int sl = a.slot[v];
+        const int sl = slots[j];
         if (do_db && fq == j && a.db) {
             float b = bacc[0] + bacc[1];
             if (sl >= 0) b += a.Lb[sl];
@@ -523,9 +533,18 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
                 const float4 p = *(const float4*)(a.acc_w + o);
                 d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
             }
-            if (a.out_bf16) *(uint2*)((bf16_t*)a.dw + o) = make_uint2(pack2bf(d[0], d[1]), pack2bf(d[2], d[3]));
+            if (a.out_bf16) *(uint2*)(patch + (16 * j + fr) * PITCH + (16 * i + 4 * fq) * 2) =
+                    make_uint2(pack2bf(d[0], d[1]), pack2bf(d[2], d[3]));
             else *(float4*)((float*)a.dw + o) = make_float4(d[0], d[1], d[2], d[3]);
         }
+    }
+    if (!a.out_bf16) return;
+    constexpr int CPR = BA / WA / 8;
+#pragma unroll 4
+    for (int u = lane; u < (BB / WB) * CPR; u += 64) {
+        const int v = v0 + wb * (BB / WB) + u / CPR, k = k0 + wa * (BA / WA) + u % CPR * 8;
+        if (v < a.V && k < a.K)
+            *(uint4*)((bf16_t*)a.dw + (long)v * a.K + k) = *(const uint4*)(patch + u / CPR * PITCH + u % CPR * 16);
     }
 }
 
@@ -561,18 +580,24 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
     p.wave_cols = cols[p.lt];
     p.nst = ce_cdiv(p.Vp, ba[p.lt]) * (ba[p.lt] / p.wave_cols);      // the tiles cover E's zero columns too
-    p.xt = p.R <= 32 ? 2 : ((long)ce_cdiv(p.R, 256) * ce_cdiv(K, 256) < 64 ? 1 : 0);
-    if (force_tile >= 0 && force_tile / 10 % 10 < 3) p.xt = force_tile / 10 % 10;
+    // dx: the tile and the number of splits over the classes by their estimated time: whole rounds of the chip (one 256 x
+    // 256 block or two 128 x 128 / four 128 x 32 blocks per CU) of 64-deep steps plus a block's start and end, and the
+    // splits' fp32 partial sums written and read once
     {
-        static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32};
-        const long tiles = (long)ce_cdiv(K, xa[p.xt]) * ce_cdiv(p.R, xb[p.xt]);
-        const int steps = ce_cdiv(V, 64);
-        long ns = (p.xt == 0 ? 256 : 512) / (tiles > 0 ? tiles : 1);
-        if (ns > steps / 4) ns = steps / 4;
-        if (ns > 64) ns = 64;
-        if (ns < 1) ns = 1;
-        p.per = ce_cdiv(steps, ns) * 64;
-        p.ns = ce_cdiv(V, p.per);
+        static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32}, slots[3] = {256, 512, 1024};
+        static const double step_us[3] = {1.75, 1.05, 0.7}, ends = 4.0;
+        const int steps = ce_cdiv(V, 64), forced = force_tile >= 0 ? force_tile / 10 % 10 : 9;
+        double best = 0;
+        for (int t = 0; t < 3; ++t) {
+            if (forced < 3 ? t != forced : (t == 2) != (p.R <= 32)) continue;
+            const long tiles = (long)ce_cdiv(K, xa[t]) * ce_cdiv(p.R, xb[t]);
+            for (int ns = 1; ns <= 64 && (ns == 1 || ns <= steps / 4); ++ns) {
+                const int per = ce_cdiv(steps, ns), n = ce_cdiv(steps, per);
+                const double rounds = (double)ce_cdiv(tiles * n, slots[t]);
+                const double us = rounds * (per + ends) * step_us[t] + (n > 1 ? 4.0 + n * 8.0 * p.R * K / 4.5e6 : 0.0);
+                if (best == 0 || us < best) { best = us; p.xt = t; p.ns = n; p.per = per * 64; }
+            }
+        }
     }
     p.wt = (long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1;
     if (force_tile >= 0 && force_tile / 100 % 10 < 2) p.wt = force_tile / 100 % 10;
@@ -593,13 +618,13 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
 
 template <int BA, int BB, int WA, int WB, int STAGES, bool STORE>
 static int launch_logits(CeLogitsArgs& a, hipStream_t s) {
-    using T = GtTile<BA, BB, WA, WB, false, false, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, false, false, STAGES, GT_PLAIN>;
     size_t lds = T::LDS_BYTES, out = (size_t)BB * (BA * 2 + 16);
     if (STORE && out > lds) lds = out;
     if (a.order && 4L * a.N > (long)lds) lds = 4L * a.N;
     constexpr auto kern = ce_logits_kernel<BA, BB, WA, WB, STAGES, STORE>;
     if (int rc = gt_lds<kern>(lds)) return rc;
-    a.map = gt_make_map((a.Vp + BA - 1) / BA, (a.N + BB - 1) / BB, 8);
+    a.map = gt_make_map((a.Vp + BA - 1) / BA, (a.N + BB - 1) / BB, 1, 8);
     a.nrank = a.order ? (ce_cdiv(a.N, CE_RANK_ROWS) + 7) / 8 * 8 : 8;
     kern<<<a.nrank + gt_grid(a.map), T::NTHR, lds, s>>>(a);
     return gt_launched();
@@ -617,21 +642,23 @@ static int ce_logits(CeLogitsArgs& a, int tile, hipStream_t s) {
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 static int launch_dx(CeDxArgs& a, hipStream_t s) {
-    using T = GtTile<BA, BB, WA, WB, true, false, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, false, STAGES, GT_FENCE>;
     constexpr auto kern = ce_dx_kernel<BA, BB, WA, WB, STAGES>;
     if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
-    a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, 8);
-    kern<<<dim3(gt_grid(a.map), a.nsplit), T::NTHR, T::LDS_BYTES, s>>>(a);
+    a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, a.nsplit, 8);
+    kern<<<gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
     return gt_launched();
 }
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 static int launch_dw(CeDwArgs& a, hipStream_t s) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
     constexpr auto kern = ce_dw_kernel<BA, BB, WA, WB, STAGES>;
-    if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
-    a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, 4);
-    kern<<<gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
+    const size_t out = (size_t)T::NW * (BB / WB) * (BA / WA * 2 + 16);
+    const size_t lds = a.out_bf16 && out > T::LDS_BYTES ? out : T::LDS_BYTES;
+    if (int rc = gt_lds<kern>(lds)) return rc;
+    a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, 1, 4);
+    kern<<<gt_grid(a.map), T::NTHR, lds, s>>>(a);
     return gt_launched();
 }
 

@@ -143,7 +143,14 @@ struct GtFrag {
 
 // The block's tile: BA x BB outputs, WA x WB waves.  Lane (fr, fq) of fragment pair (i, j) holds
 // D[wave_a0 + 16 i + 4 fq + e][wave_b0 + 16 j + fr], e = 0..3.
-template <int BA, int BB, int WA, int WB, bool TA, bool TB, int STAGES>
+// SCHED: what keeps the fragment reads and the matrix instructions of a half step apart.  One box, 8192 x 4096 x 32768,
+// TFLOP/s of the three products (row x row, column x row, column x column order), each DMA split as below:
+//   0 nothing            1258  1278  1080
+//   1 raised priority    1210  1236  1221
+//   2 scheduling fence   1184  1306  1200
+enum GtSched { GT_PLAIN = 0, GT_PRIO = 1, GT_FENCE = 2 };
+
+template <int BA, int BB, int WA, int WB, bool TA, bool TB, int STAGES, int SCHED>
 struct GtTile {
     static constexpr int NW = WA * WB, NTHR = 64 * NW;
     static constexpr int NA = BA / WA / 16, NB = BB / WB / 16;
@@ -184,8 +191,9 @@ struct GtTile {
             // this wave's share of step s has landed and its reads of the buffer that is refilled below have returned;
             // the barrier makes both true of every wave
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * P) : "memory");
+            // A's DMA here, B's between the half steps: issued together (eight instructions on a full queue) they held up
+            // the first fragment reads of the step; 4 - 9 % on all three products
             sa.issue(lds0 + nxt * STAGE_BYTES, wave);
-            sb.issue(lds0 + nxt * STAGE_BYTES + SA::BYTES, wave);
             const char* ta = smem + cur * STAGE_BYTES;
             const char* tb = ta + SA::BYTES;
 #pragma unroll
@@ -195,14 +203,16 @@ struct GtTile {
                 for (int i = 0; i < NA; ++i) av[i] = fa.load(ta, i, kk, wa * (BA / WA / 16));
 #pragma unroll
                 for (int j = 0; j < NB; ++j) bv[j] = fb.load(tb, j, kk, wb * (BB / WB / 16));
-                __builtin_amdgcn_s_setprio(1);
+                if (SCHED == GT_FENCE) __builtin_amdgcn_sched_barrier(0);
+                if (SCHED == GT_PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
                     for (int i = 0; i < NA; ++i)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[i], bv[j], acc[i][j], 0, 0, 0);
-                __builtin_amdgcn_s_setprio(0);
+                if (SCHED == GT_PRIO) __builtin_amdgcn_s_setprio(0);
                 per_half(s * GT_BK + kk * 32, bv);
+                if (kk == 0) sb.issue(lds0 + nxt * STAGE_BYTES + SA::BYTES, wave);
             }
             if (++cur == STAGES) cur = 0;
             if (++nxt == STAGES) nxt = 0;
@@ -212,13 +222,17 @@ struct GtTile {
 };
 
 // Blocks are numbered so that one XCD (hardware index = id % 8, each with its own L2) works on neighbouring tiles: it
-// owns a contiguous share of a linear order that walks strips `gb` tiles wide in b, a outermost inside a strip.
-struct GtMap { int na, nb, gb; };
-__device__ __forceinline__ bool gt_map(const GtMap& m, int id, int& ta, int& tb) {
-    const int total = m.na * m.nb;
+// owns a contiguous share of a linear order that walks the reduction's splits, inside a split strips `gb` tiles wide in
+// b, a outermost inside a strip.  (Split outermost: an XCD then reads its slice of both operands once.  With the splits
+// in the grid's y the input gradient of 1237 x 776 x 30011 took 96 us instead of 73.)
+struct GtMap { int na, nb, ns, gb; };
+__device__ __forceinline__ bool gt_map(const GtMap& m, int id, int& ta, int& tb, int& split) {
+    const int tiles = m.na * m.nb, total = tiles * m.ns;
     const int per = (total + 7) >> 3;
-    const int lin = (id & 7) * per + (id >> 3);
+    int lin = (id & 7) * per + (id >> 3);
     if ((id >> 3) >= per || lin >= total) return false;
+    split = lin / tiles;
+    lin -= split * tiles;
     const int strip = lin / (m.na * m.gb);
     const int w = min(m.gb, m.nb - strip * m.gb);
     const int in = lin - strip * m.na * m.gb;
@@ -228,11 +242,11 @@ __device__ __forceinline__ bool gt_map(const GtMap& m, int id, int& ta, int& tb)
 }
 
 // ---- host side
-static inline GtMap gt_make_map(int na, int nb, int gb) {
-    GtMap m; m.na = na; m.nb = nb; m.gb = gb < nb ? gb : nb;
+static inline GtMap gt_make_map(int na, int nb, int ns, int gb) {
+    GtMap m; m.na = na; m.nb = nb; m.ns = ns; m.gb = gb < nb ? gb : nb;
     return m;
 }
-static inline unsigned gt_grid(const GtMap& m) { return (unsigned)(((long)m.na * m.nb + 7) / 8 * 8); }
+static inline unsigned gt_grid(const GtMap& m) { return (unsigned)(((long)m.na * m.nb * m.ns + 7) / 8 * 8); }
 
 // dynamic LDS above 64 KiB has to be asked for, once per kernel and device
 template <auto Kern>
