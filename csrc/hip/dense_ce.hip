@@ -184,27 +184,9 @@ struct CeRowsArgs {
     int N, V, K, Vp;
     bf16_t* E; const bf16_t* x; bf16_t* xs;           // xs = bf16(g x)
     float* rows; CeRow* row; bf16_t* g2; int g2_pitch;      // g2[0] + g2[1] = g in two bf16 terms, zero behind row N
+    float* loss;                     // scoring a single row: its loss is the mean
 };
 
-__device__ __forceinline__ float ce_block_max(float v, float* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) r = fmaxf(r, red[w]);
-    __syncthreads();
-    return r;
-}
-__device__ __forceinline__ float ce_block_sum(float v, float* red) {
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) r += red[w];
-    __syncthreads();
-    return r;
-}
 // 2^d for whole d, exact (0 below the normal range: such a term is 2^-126 of the row's largest)
 __device__ __forceinline__ float ce_pow2(float d) { return d < -126.f ? 0.f : ldexpf(1.f, (int)d); }
 
@@ -214,51 +196,69 @@ __device__ __forceinline__ float ce_row_loss(float cref, float S, float zt) {
     return lse < INFINITY ? lse - zt : NAN;
 }
 
-template <bool GRAD>
-__global__ __launch_bounds__(256) void ce_rows_kernel(const CeRowsArgs a) {
-    __shared__ float red[4];
+// (reference, sum) of a row's tiles: running maximum and sum, entries with sum 0 (no class) left out
+struct CeSum {
+    float c, s, lo;                                           // lo: the smallest reference seen
+    __device__ __forceinline__ void add(float oc, float os, float olo) {
+        if (os == 0.f) return;
+        const float m = fmaxf(c, oc);
+        s = (s == 0.f ? 0.f : (c == m ? s : s * ce_pow2(c - m))) + (oc == m ? os : os * ce_pow2(oc - m));
+        c = m;
+        lo = fminf(lo, olo);
+    }
+    __device__ __forceinline__ void wave() {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) add(__shfl_xor(c, o, 64), __shfl_xor(s, o, 64), __shfl_xor(lo, o, 64));
+    }
+};
+
+template <bool GRAD, int NTHR>
+__global__ __launch_bounds__(NTHR) void ce_rows_kernel(const CeRowsArgs a) {
+    __shared__ float red[NTHR / 64][3];
     const int r = blockIdx.x, tid = threadIdx.x;
     if (GRAD && r == 0)
-        for (int i = a.N + tid; i < a.g2_pitch; i += 256) a.g2[i] = a.g2[a.g2_pitch + i] = 0;
+        for (int i = a.N + tid; i < a.g2_pitch; i += NTHR) a.g2[i] = a.g2[a.g2_pitch + i] = 0;
     const long lab = a.labels[r];
     const bool live = (unsigned long)lab < (unsigned long)a.V;
     if (!live) {
-        if (tid == 0) a.rows[r] = lab < 0 ? 0.f : NAN;        // a label past the last class is an error, not padding
+        const float v = lab < 0 ? 0.f : NAN;                  // a label past the last class is an error, not padding
+        if (tid == 0) {
+            a.rows[r] = v;
+            if (a.loss) *a.loss = v;
+        }
         if (GRAD) {
             if (tid == 0) { a.row[r] = CeRow{0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}}; a.g2[r] = 0; a.g2[a.g2_pitch + r] = 0; }
-            for (int k = tid * 8; k < a.K; k += 256 * 8) *(uint4*)(a.xs + (long)r * a.K + k) = make_uint4(0, 0, 0, 0);
+            for (int k = tid * 8; k < a.K; k += NTHR * 8) *(uint4*)(a.xs + (long)r * a.K + k) = make_uint4(0, 0, 0, 0);
         }
         return;
     }
     const float2* st = a.stats + (long)r * a.nst;
-    float cref = -INFINITY;
-    for (int t = tid; t < a.nst; t += 256) {
-        const float2 v = st[t];
-        if (v.y != 0.f) cref = fmaxf(cref, v.x);
+    CeSum t = {-INFINITY, 0.f, INFINITY};
+    for (int i = tid; i < a.nst; i += NTHR) {
+        const float2 v = st[i];
+        t.add(v.x, v.y, v.x);
     }
-    cref = ce_block_max(cref, red);
-    if (cref == -INFINITY) cref = 0.f;                        // no class left: S = 0
-    float S = 0.f;
-    int other = 0;                                            // a tile with a reference of its own
-    for (int t = tid; t < a.nst; t += 256) {
-        const float2 v = st[t];
-        if (v.y == 0.f) continue;
-        S += v.x == cref ? v.y : v.y * ce_pow2(v.x - cref);
-        other |= v.x != cref;
-    }
-    S = ce_block_sum(S, red);
+    t.wave();
+    if ((tid & 63) == 0) { red[tid >> 6][0] = t.c; red[tid >> 6][1] = t.s; red[tid >> 6][2] = t.lo; }
+    __syncthreads();
+    t = {red[0][0], red[0][1], red[0][2]};
+    for (int w = 1; w < NTHR / 64; ++w) t.add(red[w][0], red[w][1], red[w][2]);
+    const float cref = t.s == 0.f ? 0.f : t.c, S = t.s;       // no class left: S = 0
     const float zt = a.zt[r];
     const float loss = ce_row_loss(cref, S, zt);
-    if (tid == 0) a.rows[r] = loss;
+    if (tid == 0) {
+        a.rows[r] = loss;
+        if (a.loss) *a.loss = loss;
+    }
     if (!GRAD) return;
     bf16_t* E = a.E + (long)r * a.Vp;
-    if (__syncthreads_or(other)) {                            // bring those tiles to the row's reference
-        for (int t = 0; t < a.nst; ++t) {
-            const float2 v = st[t];
+    if (t.s != 0.f && t.lo != cref) {                         // bring the tiles with a reference of their own to the row's
+        for (int i = 0; i < a.nst; ++i) {
+            const float2 v = st[i];
             if (v.y == 0.f || v.x == cref) continue;
             const float f = ce_pow2(v.x - cref);
-            const int v1 = min((t + 1) * a.wave_cols, a.V);
-            for (int c = t * a.wave_cols + tid; c < v1; c += 256) E[c] = f2bf(bf2f(E[c]) * f);
+            const int v1 = min((i + 1) * a.wave_cols, a.V);
+            for (int c = i * a.wave_cols + tid; c < v1; c += NTHR) E[c] = f2bf(bf2f(E[c]) * f);
         }
         __syncthreads();                                      // the label's entry is written below
     }
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const CeRowsArgs a) {
         a.g2[r] = hi;
         a.g2[a.g2_pitch + r] = lo;
     }
-    for (int k = tid * 8; k < a.K; k += 256 * 8) {
+    for (int k = tid * 8; k < a.K; k += NTHR * 8) {
         float f[8];
         unpack8(*(const uint4*)(a.x + (long)r * a.K + k), f);
 #pragma unroll
@@ -303,8 +303,9 @@ __global__ __launch_bounds__(1024) void ce_mean_kernel(const float* rows, const 
 }
 
 // Scoring a few rows of few tiles: row losses (a wave each) and their mean in one block instead of two launches.  With
-// 65536 statistics (32 rows of 65536 classes) the one block took 40 us and the two launches 6; below 4096 it is shorter.
-#define CE_FEW 4096
+// 2048 statistics for each of 32 rows the one block took 40 us and the two launches 6; it is for short ones only.
+#define CE_FEW_STATS 256
+#define CE_FEW_ROWS 32
 __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, float* loss) {
     const int lane = threadIdx.x & 63;
     for (int r = threadIdx.x >> 6; r < a.N; r += 16) {
@@ -312,19 +313,13 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
         float v = lab < 0 ? 0.f : NAN;
         if ((unsigned long)lab < (unsigned long)a.V) {
             const float2* st = a.stats + (long)r * a.nst;
-            float cref = -INFINITY, S = 0.f;
-            for (int t = lane; t < a.nst; t += 64) {
-                const float2 p = st[t];
-                if (p.y != 0.f) cref = fmaxf(cref, p.x);
+            CeSum t = {-INFINITY, 0.f, INFINITY};
+            for (int i = lane; i < a.nst; i += 64) {
+                const float2 p = st[i];
+                t.add(p.x, p.y, p.x);
             }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) cref = fmaxf(cref, __shfl_xor(cref, o, 64));
-            if (cref == -INFINITY) cref = 0.f;
-            for (int t = lane; t < a.nst; t += 64) {
-                const float2 p = st[t];
-                if (p.y != 0.f) S += p.x == cref ? p.y : p.y * ce_pow2(p.x - cref);
-            }
-            v = ce_row_loss(cref, wave_sum(S), a.zt[r]);
+            t.wave();
+            v = ce_row_loss(t.s == 0.f ? 0.f : t.c, t.s, a.zt[r]);
         }
         if (lane == 0) a.rows[r] = v;
     }
@@ -548,6 +543,127 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     }
 }
 
+// dw for at most 64 rows: one step of the reduction, so the kernel is its store (2 or 4 K V bytes) and what feeds it.  A
+// wave keeps the E fragments of its 32 classes in registers and walks its share of the features (all of them, or fewer
+// when the classes alone do not make three blocks per CU) 64 at a time, x' through two LDS buffers (L2 serves it, every
+// block reads the same 64 x K).  131072 classes x 4096: 286 us where the tile product above took 312 - 362; 50000 x 1024: 33
+// and 40.  The store counts as a memory
+// operation like the DMA: waiting for the next chunk leaves the STORES youngest operations, this chunk's stores, in
+// flight, which holds because every one of them is issued (out of range: past the descriptor, dropped).
+template <bool BF16>
+__global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
+    constexpr int BV = 128, WV = 32, KC = 64, ES = BF16 ? 2 : 4, PITCH = KC * ES + 16;
+    constexpr int STORES = WV * KC * ES / 16 / 64;
+    using SE = GtStage<BV, 4, true>;
+    using SX = GtStage<KC, 4, true>;
+    constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > SE::BYTES ? PATCH : SE::BYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];                       // [E, later the patches][x'][x']
+    const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int v0 = blockIdx.x * BV, wv = v0 + wave * WV;
+    const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)smem;
+    char* xbuf = smem + E_OR_PATCH;
+    SE se;
+    se.init(a.e, v0, 0, a.N, wave, lane);
+    se.issue(lds0, wave);
+    int slots[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) slots[j] = wv + 16 * j + fr < a.V ? a.slot[wv + 16 * j + fr] : -1;
+    auto fetch = [&](int k, int buf) {
+        SX sx;
+        sx.init(a.xs, k, 0, a.N, wave, lane);
+        sx.issue(lds0 + E_OR_PATCH + buf * SX::BYTES, wave);
+        asm volatile("" ::: "memory");                       // the stores of this chunk stay behind the DMA of the next
+    };
+    const int nc = (a.K + KC - 1) / KC, share = (nc + gridDim.y - 1) / gridDim.y;
+    const int c0 = blockIdx.y * share, c1 = min(c0 + share, nc);
+    fetch(c0 * KC, c0 & 1);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    GtFrag<BV, true> fe;
+    GtFrag<KC, true> fx;
+    fe.init(wave * WV, lane);
+    fx.init(0, lane);
+    bf16x8_t ev[2][2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ev[kk][j] = fe.load(smem, j, kk, wave * (WV / 16));
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");                 // E's LDS becomes the patches
+
+    if (a.db && c0 == 0) {
+        f32x4 b = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + kk * 32 + 8 * fq);
+            const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, (fr & ~1) == 4 * j ? gv : z),
+                                                            ev[kk][j], b, 0, 0, 0);
+        }
+        const int v = wv + 16 * fq + fr;
+        if (fq < 2 && v < a.V) {
+            float t = b[0] + b[1];
+            const int sl = fq == 0 ? slots[0] : slots[1];
+            if (sl >= 0) t += a.Lb[sl];
+            if (a.acc_b) t += a.acc_b[v];
+            if (BF16) ((bf16_t*)a.db)[v] = f2bf(t);
+            else ((float*)a.db)[v] = t;
+        }
+    }
+
+    char* patch = smem + wave * WV * PITCH;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((char*)a.dw + (long)v0 * a.K * ES, 0, 0x7FFFFFF0,
+                                                                        0x00020000);
+    for (int c = c0; c < c1; ++c) {
+        if (c > c0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(STORES) : "memory");
+        fetch((c + 1) * KC, (c + 1) & 1);                     // past the share unused, past the last feature zeros
+        const char* xt = xbuf + (c & 1) * SX::BYTES;
+        f32x4 acc[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bf16x8_t xv = fx.load(xt, i, kk, 0);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, ev[kk][j], acc[i][j], 0, 0, 0);
+            }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int v = wv + 16 * j + fr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = c * KC + 16 * i + 4 * fq;
+                f32x4 d = acc[i][j];
+                if (slots[j] >= 0 && k < a.K) {
+                    const float4 p = *(const float4*)(a.L + (long)slots[j] * a.K + k);
+                    d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
+                }
+                if (a.acc_w && v < a.V && k < a.K) {
+                    const float4 p = *(const float4*)(a.acc_w + (long)v * a.K + k);
+                    d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
+                }
+                char* o = patch + (16 * j + fr) * PITCH + (16 * i + 4 * fq) * ES;
+                if (BF16) *(uint2*)o = make_uint2(pack2bf(d[0], d[1]), pack2bf(d[2], d[3]));
+                else *(f32x4*)o = d;
+            }
+        }
+        constexpr int CPR = KC * ES / 16;                     // 16-byte groups per class
+        typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int t = 0; t < STORES; ++t) {
+            const int u = t * 64 + lane, row = u / CPR, g = u % CPR;
+            const int k = c * KC + g * (16 / ES);
+            const unsigned off = (wv + row < a.V && k < a.K) ? (unsigned)(((wave * WV + row) * a.K + k) * ES) : GT_OOB;
+            __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t*)(patch + row * PITCH + g * 16), rs, off, 0, 0);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the last fetch has landed before the LDS is given back
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 #define CE_MAX_ROWS 8192      // rows of a piece (their labels are ranked in 32 KiB of LDS)
 
@@ -600,7 +716,8 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         }
     }
     p.wt = (long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1;
-    if (force_tile >= 0 && force_tile / 100 % 10 < 2) p.wt = force_tile / 100 % 10;
+    if (p.R <= 64) p.wt = 2;
+    if (force_tile >= 0 && force_tile / 100 % 10 < (p.R <= 64 ? 3 : 2)) p.wt = force_tile / 100 % 10;
     p.g2_pitch = ce_cdiv(p.R, 64) * 64;
     long o = 0;
     auto take = [&](long bytes) { const long at = o; o += (bytes + 255) / 256 * 256; return at; };
@@ -662,6 +779,14 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     return gt_launched();
 }
 
+template <bool BF16>
+static int launch_dw_thin(CeDwArgs& a, hipStream_t s) {
+    const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = 128 * 64 * 2;
+    const int nv = (a.V + 127) / 128, nc = (a.K + 63) / 64, want = (768 + nv - 1) / nv;
+    ce_dw_thin_kernel<BF16><<<dim3(nv, want < nc ? want : nc), 256, (patch > e ? patch : e) + 2 * 64 * 64 * 2, s>>>(a);
+    return gt_launched();
+}
+
 static bool ce_range_ok(int N, int V, int K) {
     // 64 k rows or 256 rows of any operand within 31 bits of byte offset
     return N > 0 && V > 0 && K > 0 && (K & 7) == 0 && (long)K * 512 < (1L << 31) && ((long)V + 64) * 512 < (1L << 31) &&
@@ -706,17 +831,21 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         CeRowsArgs b;
         b.stats = a.stats; b.nst = p.nst; b.wave_cols = p.wave_cols; b.zt = zt; b.labels = a.labels; b.count = count;
         b.N = n; b.V = V; b.K = K; b.Vp = p.Vp; b.E = E; b.x = a.x.p; b.xs = xs; b.rows = rows + r0;
-        b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch;
+        b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch; b.loss = nullptr;
+        const bool wide = n <= 256 && p.nst > 512;            // few long rows: 1024 threads each (16 -> 6 us at 4096 entries)
         if (!train) {
-            if ((long)n * p.nst <= CE_FEW) {
+            if (n <= CE_FEW_ROWS && p.nst <= CE_FEW_STATS) {
                 ce_score_few_kernel<<<1, 1024, 0, s>>>(b, loss);
                 return gt_launched();
             }
-            ce_rows_kernel<false><<<n, 256, 0, s>>>(b);
-            ce_mean_kernel<<<1, 1024, 0, s>>>(rows, count, N, loss);
+            if (n == 1) b.loss = loss;
+            if (wide) ce_rows_kernel<false, 1024><<<n, 1024, 0, s>>>(b);
+            else ce_rows_kernel<false, 256><<<n, 256, 0, s>>>(b);
+            if (n > 1) ce_mean_kernel<<<1, 1024, 0, s>>>(rows, count, N, loss);
             return gt_launched();
         }
-        ce_rows_kernel<true><<<n, 256, 0, s>>>(b);
+        if (wide) ce_rows_kernel<true, 1024><<<n, 1024, 0, s>>>(b);
+        else ce_rows_kernel<true, 256><<<n, 256, 0, s>>>(b);
 
         CeLabelsArgs l;
         l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot;
@@ -751,7 +880,11 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         c.out_bf16 = out_bf16 && last;
         c.dw = last ? dw : (void*)aw;
         c.db = db ? (last ? db : (void*)ab) : nullptr;
-        rc = p.wt == 0 ? launch_dw<256, 256, 2, 4, 2>(c, s) : launch_dw<128, 128, 2, 2, 2>(c, s);
+        switch (p.wt) {
+            case 0: rc = launch_dw<256, 256, 2, 4, 2>(c, s); break;
+            case 1: rc = launch_dw<128, 128, 2, 2, 2>(c, s); break;
+            default: rc = c.out_bf16 ? launch_dw_thin<true>(c, s) : launch_dw_thin<false>(c, s);
+        }
         if (rc) return rc;
     }
     return gt_launched();

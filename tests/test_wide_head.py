@@ -181,7 +181,7 @@ def test_score(N, K, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tile", [0, 1, 2, 3, 109, 119, 129, 9, 19, 29])
-@pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (260, 136, 600)])
+@pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (64, 328, 500), (260, 136, 600)])
 def test_every_tile(tile, N, K, V, monkeypatch):
     from distributeddeeplearning_amd.ops import hip
     monkeypatch.setattr(hip, "CE_TILE", tile)
@@ -266,9 +266,10 @@ def test_row_pieces(N, dtype, monkeypatch):
     from distributeddeeplearning_amd.ops import hip
     a = make(N, 72, 700, seed=N, drop=0.1)
     d = cuda(*a)
-    monkeypatch.setattr(hip, "CE_PIECE_BYTES", 256 * 704 * 2)
-    out = F.dense_softmax_ce(*d, grad_dtype=dtype)
-    check(out, exact(*a), dtype)
+    for piece in (256, 64):
+        monkeypatch.setattr(hip, "CE_PIECE_BYTES", piece * 704 * 2)
+        out = F.dense_softmax_ce(*d, grad_dtype=dtype)
+        check(out, exact(*a), dtype)
 
 
 @pytest.mark.gpu
