@@ -543,20 +543,21 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     }
 }
 
-// dw for at most 64 rows: one step of the reduction, so the kernel is its store (2 or 4 K V bytes) and what feeds it.  A
+// dw for at most 64 NS rows, NS = 1 or 2 steps of the reduction: the kernel is its store (2 or 4 K V bytes) and what feeds
+// it.  A
 // wave keeps the E fragments of its 32 classes in registers and walks its share of the features (all of them, or fewer
 // when the classes alone do not make three blocks per CU) 64 at a time, x' through two LDS buffers (L2 serves it, every
-// block reads the same 64 x K).  131072 classes x 4096: 286 us where the tile product above took 312 - 362; 50000 x 1024: 33
-// and 40.  The store counts as a memory
+// block reads the same 64 x K).  64 x 2048 x 30000: 32 us, 3.9 TB/s of stores, where the tile product above took 47; 8 x
+// 1024 x 50000: 24 and 40.  The store counts as a memory
 // operation like the DMA: waiting for the next chunk leaves the STORES youngest operations, this chunk's stores, in
 // flight, which holds because every one of them is issued (out of range: past the descriptor, dropped).
-template <bool BF16>
-__global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
+template <bool BF16, int NS>
+__global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const CeDwArgs a) {
     constexpr int BV = 128, WV = 32, KC = 64, ES = BF16 ? 2 : 4, PITCH = KC * ES + 16;
     constexpr int STORES = WV * KC * ES / 16 / 64;
     using SE = GtStage<BV, 4, true>;
     using SX = GtStage<KC, 4, true>;
-    constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > SE::BYTES ? PATCH : SE::BYTES;
+    constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > NS * SE::BYTES ? PATCH : NS * SE::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];                       // [E, later the patches][x'][x']
     const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -565,14 +566,16 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
     char* xbuf = smem + E_OR_PATCH;
     SE se;
     se.init(a.e, v0, 0, a.N, wave, lane);
-    se.issue(lds0, wave);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) se.issue(lds0 + n * SE::BYTES, wave);
     int slots[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) slots[j] = wv + 16 * j + fr < a.V ? a.slot[wv + 16 * j + fr] : -1;
     auto fetch = [&](int k, int buf) {
         SX sx;
         sx.init(a.xs, k, 0, a.N, wave, lane);
-        sx.issue(lds0 + E_OR_PATCH + buf * SX::BYTES, wave);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) sx.issue(lds0 + E_OR_PATCH + (buf * NS + n) * SX::BYTES, wave);
         asm volatile("" ::: "memory");                       // the stores of this chunk stay behind the DMA of the next
     };
     const int nc = (a.K + KC - 1) / KC, share = (nc + gridDim.y - 1) / gridDim.y;
@@ -583,19 +586,19 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
     GtFrag<KC, true> fx;
     fe.init(wave * WV, lane);
     fx.init(0, lane);
-    bf16x8_t ev[2][2];
+    bf16x8_t ev[2 * NS][2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2 * NS; ++kk)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) ev[kk][j] = fe.load(smem, j, kk, wave * (WV / 16));
+        for (int j = 0; j < 2; ++j) ev[kk][j] = fe.load(smem + (kk >> 1) * SE::BYTES, j, kk & 1, wave * (WV / 16));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");                 // E's LDS becomes the patches
 
     if (a.db && c0 == 0) {
         f32x4 b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + kk * 32 + 8 * fq);
+        for (int kk = 0; kk < 2 * NS; ++kk) {
             const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            const s16x8 gv = kk * 32 < a.g2_pitch ? *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + kk * 32 + 8 * fq) : z;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
                 b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, (fr & ~1) == 4 * j ? gv : z),
@@ -618,15 +621,15 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
     for (int c = c0; c < c1; ++c) {
         if (c > c0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(STORES) : "memory");
         fetch((c + 1) * KC, (c + 1) & 1);                     // past the share unused, past the last feature zeros
-        const char* xt = xbuf + (c & 1) * SX::BYTES;
+        const char* xt = xbuf + (c & 1) * NS * SX::BYTES;
         f32x4 acc[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int kk = 0; kk < 2 * NS; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bf16x8_t xv = fx.load(xt, i, kk, 0);
+                const bf16x8_t xv = fx.load(xt + (kk >> 1) * SX::BYTES, i, kk & 1, 0);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, ev[kk][j], acc[i][j], 0, 0, 0);
@@ -715,9 +718,11 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
             }
         }
     }
-    p.wt = (long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1;
-    if (p.R <= 64) p.wt = 2;
-    if (force_tile >= 0 && force_tile / 100 % 10 < (p.R <= 64 ? 3 : 2)) p.wt = force_tile / 100 % 10;
+    // dw: the streaming kernel to 128 rows (100 x 1024 x 20000: 24 us, 128 x 4096 x 50000: 171, where the tiles took 28 and
+    // 203; with four steps, 200 x 1024 x 20000: 37 and 37, 256 x 2048 x 50000: 143 and 123)
+    p.wt = p.R <= 128 ? 2 : ((long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1);
+    if (force_tile >= 0 && force_tile / 100 % 10 < 2) p.wt = force_tile / 100 % 10;
+    if (p.wt == 2 && p.R > 64) p.wt = 3;
     p.g2_pitch = ce_cdiv(p.R, 64) * 64;
     long o = 0;
     auto take = [&](long bytes) { const long at = o; o += (bytes + 255) / 256 * 256; return at; };
@@ -779,11 +784,13 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     return gt_launched();
 }
 
-template <bool BF16>
+template <bool BF16, int NS>
 static int launch_dw_thin(CeDwArgs& a, hipStream_t s) {
-    const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = 128 * 64 * 2;
+    const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = NS * 128 * 64 * 2, lds = (patch > e ? patch : e) + NS * 2 * 64 * 64 * 2;
+    constexpr auto kern = ce_dw_thin_kernel<BF16, NS>;
+    if (int rc = gt_lds<kern>(lds)) return rc;
     const int nv = (a.V + 127) / 128, nc = (a.K + 63) / 64, want = (768 + nv - 1) / nv;
-    ce_dw_thin_kernel<BF16><<<dim3(nv, want < nc ? want : nc), 256, (patch > e ? patch : e) + 2 * 64 * 64 * 2, s>>>(a);
+    kern<<<dim3(nv, want < nc ? want : nc), 256, lds, s>>>(a);
     return gt_launched();
 }
 
@@ -883,7 +890,8 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         switch (p.wt) {
             case 0: rc = launch_dw<256, 256, 2, 4, 2>(c, s); break;
             case 1: rc = launch_dw<128, 128, 2, 2, 2>(c, s); break;
-            default: rc = c.out_bf16 ? launch_dw_thin<true>(c, s) : launch_dw_thin<false>(c, s);
+            case 2: rc = c.out_bf16 ? launch_dw_thin<true, 1>(c, s) : launch_dw_thin<false, 1>(c, s); break;
+            default: rc = c.out_bf16 ? launch_dw_thin<true, 2>(c, s) : launch_dw_thin<false, 2>(c, s);
         }
         if (rc) return rc;
     }

@@ -181,7 +181,7 @@ def test_score(N, K, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tile", [0, 1, 2, 3, 109, 119, 129, 9, 19, 29])
-@pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (64, 328, 500), (260, 136, 600)])
+@pytest.mark.parametrize("N,K,V", [(37, 72, 1030), (64, 328, 500), (128, 136, 333), (190, 136, 400), (260, 136, 600)])
 def test_every_tile(tile, N, K, V, monkeypatch):
     from distributeddeeplearning_amd.ops import hip
     monkeypatch.setattr(hip, "CE_TILE", tile)
