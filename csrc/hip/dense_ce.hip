@@ -329,22 +329,21 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
 
 // ------------------------------------------------------------------------------------------------ 3. label terms
 // Sorted position i starts a class: its rows i, i + 1, .. (ascending) are summed into L[first row] and slot[class] is set
-// to it.  Eight features per thread.  Block (n, 0), behind the positions, takes the mean of the row losses.
+// to it.  Eight features per thread, 256 threads.  Position n, behind them all, takes the mean of the row losses.
 struct CeLabelsArgs {
     const CeRow* row; const int* order; const bf16_t* x; const bf16_t* xs; int N, K;
     int* slot; float* L; float* Lb;                          // [N][K], [N]
     const float* rows_all; const float* count; int n_all; float* loss;      // loss nullptr: not the last piece
 };
 
-__global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) {
-    const int i = blockIdx.x;
+__device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chunk) {
     if (i == a.N) {
-        if (a.loss && blockIdx.y == 0) ce_mean<256>(a.rows_all, a.count, a.n_all, a.loss);
+        if (a.loss && chunk == 0) ce_mean<256>(a.rows_all, a.count, a.n_all, a.loss);
         return;
     }
     const int first = a.order[i], lab = a.row[first].label;
     if (lab < 0 || (i > 0 && a.row[a.order[i - 1]].label == lab)) return;
-    const int k = (blockIdx.y * 256 + threadIdx.x) * 8, lane = threadIdx.x & 63;
+    const int k = (chunk * 256 + threadIdx.x) * 8, lane = threadIdx.x & 63;
     const bool on = k < a.K;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b = 0.f;
     for (int p = i; p < a.N; p += 64) {                       // 64 positions at a time; the class ends inside one of them
@@ -371,11 +370,12 @@ __global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) {
         *(float4*)o = make_float4(s[0], s[1], s[2], s[3]);
         *(float4*)(o + 4) = make_float4(s[4], s[5], s[6], s[7]);
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0) {
+    if (chunk == 0 && threadIdx.x == 0) {
         a.slot[lab] = first;
         a.Lb[first] = b;
     }
 }
+__global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) { ce_labels(a, blockIdx.x, blockIdx.y); }
 
 // ------------------------------------------------------------------------------------------------ 4. dx
 struct CeDxArgs {
@@ -383,6 +383,7 @@ struct CeDxArgs {
     int N, V, K;
     int nsplit, per_split;           // classes per split (a multiple of 64)
     const CeRow* row; bf16_t* dx; float* slab;    // slab [nsplit][N][K] when nsplit > 1
+    CeLabelsArgs lab; int nlab, nlab_chunks;      // few rows: the first nlab blocks (a multiple of 8) do the label terms
     GtMap map;
 };
 
@@ -404,8 +405,13 @@ template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dx_kernel(const CeDxArgs a) {
     using T = GtTile<BA, BB, WA, WB, true, false, STAGES, GT_FENCE>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    if (T::NTHR == 256 && (int)blockIdx.x < a.nlab) {
+        const int i = blockIdx.x / a.nlab_chunks;
+        if (i <= a.lab.N) ce_labels(a.lab, i, blockIdx.x - i * a.nlab_chunks);
+        return;
+    }
     int ta, tb, split;
-    if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
+    if (!gt_map(a.map, blockIdx.x - a.nlab, ta, tb, split)) return;
     const int k0 = ta * BA, r0 = tb * BB;
     const int v0 = split * a.per_split, v1 = min(v0 + a.per_split, a.V);
     f32x4 acc[T::NA][T::NB];
@@ -431,11 +437,12 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     }
 }
 
-__global__ __launch_bounds__(256) void ce_dx_finish_kernel(const float* __restrict__ slab, const CeRow* __restrict__ row,
-                                                           const bf16_t* __restrict__ w, bf16_t* __restrict__ dx, int N,
-                                                           int K, int nsplit) {
+// block b of nb (256 threads each)
+__device__ __forceinline__ void ce_dx_finish(const float* __restrict__ slab, const CeRow* __restrict__ row,
+                                             const bf16_t* __restrict__ w, bf16_t* __restrict__ dx, int N, int K, int nsplit,
+                                             int b, int nb) {
     const long MK = (long)N * K;
-    for (long i = (blockIdx.x * 256L + threadIdx.x) * 4; i < MK; i += gridDim.x * 1024L) {
+    for (long i = (b * 256L + threadIdx.x) * 4; i < MK; i += nb * 1024L) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         int k = 0;
         for (; k + 3 < nsplit; k += 4) {                       // four loads in flight, added in split order
@@ -454,6 +461,11 @@ __global__ __launch_bounds__(256) void ce_dx_finish_kernel(const float* __restri
         ce_dx_store(row[r], w, K, (int)(i - (long)r * K), d, dx + i);
     }
 }
+__global__ __launch_bounds__(256) void ce_dx_finish_kernel(const float* __restrict__ slab, const CeRow* __restrict__ row,
+                                                           const bf16_t* __restrict__ w, bf16_t* __restrict__ dx, int N,
+                                                           int K, int nsplit) {
+    ce_dx_finish(slab, row, w, dx, N, K, nsplit, blockIdx.x, gridDim.x);
+}
 
 // ------------------------------------------------------------------------------------------------ 5. dw, db
 struct CeDwArgs {
@@ -463,6 +475,8 @@ struct CeDwArgs {
     const int* slot; const float* L; const float* Lb;       // the label terms' remainders (ce_labels)
     const float* acc_w; const float* acc_b;       // earlier row pieces ([V][K], [V]) or nullptr
     void* dw; void* db; int out_bf16;             // this piece's output: fp32 (possibly the accumulator) or bf16
+    // streaming kernel: blocks nv, nv + 1, .. of the first row of the grid finish the splits of dx
+    const float* slab; const CeRow* row; const bf16_t* w; bf16_t* dx; int nsplit, nv;
     GtMap map;
 };
 
@@ -559,6 +573,11 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
     using SX = GtStage<KC, 4, true>;
     constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > NS * SE::BYTES ? PATCH : NS * SE::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];                       // [E, later the patches][x'][x']
+    if ((int)blockIdx.x >= a.nv) {
+        if (blockIdx.y == 0)
+            ce_dx_finish(a.slab, a.row, a.w, a.dx, a.N, a.K, a.nsplit, blockIdx.x - a.nv, gridDim.x - a.nv);
+        return;
+    }
     const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int v0 = blockIdx.x * BV, wv = v0 + wave * WV;
@@ -768,7 +787,12 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     constexpr auto kern = ce_dx_kernel<BA, BB, WA, WB, STAGES>;
     if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, a.nsplit, 8);
-    kern<<<gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
+    a.nlab_chunks = ce_cdiv(a.K, 2048);
+    a.nlab = 0;
+    // a launch of its own costs 4 us; in front of the tiles the label blocks hold a tile's LDS, so only while they are few
+    if (a.N <= 128 && T::NTHR == 256) a.nlab = (a.nlab_chunks * (a.N + 1) + 7) / 8 * 8;
+    else ce_labels_kernel<<<dim3(a.N + 1, a.nlab_chunks), 256, 0, s>>>(a.lab);
+    kern<<<a.nlab + gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
     return gt_launched();
 }
 
@@ -789,8 +813,10 @@ static int launch_dw_thin(CeDwArgs& a, hipStream_t s) {
     const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = NS * 128 * 64 * 2, lds = (patch > e ? patch : e) + NS * 2 * 64 * 64 * 2;
     constexpr auto kern = ce_dw_thin_kernel<BF16, NS>;
     if (int rc = gt_lds<kern>(lds)) return rc;
-    const int nv = (a.V + 127) / 128, nc = (a.K + 63) / 64, want = (768 + nv - 1) / nv;
-    kern<<<dim3(nv, want < nc ? want : nc), 256, lds, s>>>(a);
+    const int nc = (a.K + 63) / 64;
+    a.nv = (a.V + 127) / 128;
+    const int want = (768 + a.nv - 1) / a.nv, nfin = a.slab ? ce_cdiv((long)a.N * a.K, 1024) : 0;
+    kern<<<dim3(a.nv + nfin, want < nc ? want : nc), 256, lds, s>>>(a);
     return gt_launched();
 }
 
@@ -858,10 +884,10 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot;
         l.L = (float*)(ws + p.o_L); l.Lb = (float*)(ws + p.o_Lb);
         l.rows_all = rows; l.count = count; l.n_all = N; l.loss = last ? loss : nullptr;
-        ce_labels_kernel<<<dim3(n + 1, ce_cdiv(K, 2048)), 256, 0, s>>>(l);
         if (int e = gt_launched()) return e;
 
         CeDxArgs d;
+        d.lab = l;
         d.w = {w, K, K}; d.e = {E, p.Vp, n};
         d.N = n; d.V = V; d.K = K; d.nsplit = p.ns; d.per_split = p.per; d.row = row; d.dx = (bf16_t*)dx + (long)r0 * K;
         d.slab = p.ns > 1 ? (float*)(ws + p.o_slab) : nullptr;
@@ -871,13 +897,14 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
             default: rc = launch_dx<128, 32, 4, 1, 4>(d, s);
         }
         if (rc) return rc;
-        if (p.ns > 1) {
+        if (p.ns > 1 && p.wt < 2) {
             const long nb = ((long)n * K + 1023) / 1024;
             ce_dx_finish_kernel<<<(int)(nb > 2048 ? 2048 : nb), 256, 0, s>>>(d.slab, row, w, d.dx, n, K, p.ns);
         }
 
         CeDwArgs c;
         c.xs = {xs, K, K}; c.e = {E, p.Vp, p.Vp};
+        c.slab = d.slab; c.row = row; c.w = w; c.dx = d.dx; c.nsplit = p.ns; c.nv = 0;
         c.N = n; c.V = V; c.K = K; c.g2 = g2; c.g2_pitch = p.g2_pitch; c.slot = a.slot; c.L = l.L; c.Lb = l.Lb;
         // several pieces add up in fp32: in the output itself, or in the workspace until the last piece rounds
         float* aw = out_bf16 ? (float*)(ws + p.o_accw) : (float*)dw;

@@ -159,7 +159,7 @@ struct GtTile {
     static constexpr int STAGE_BYTES = SA::BYTES + SB::BYTES;
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
     static constexpr int P = SA::P + SB::P;
-    static_assert(NA >= 1 && NB >= 1 && LDS_BYTES <= 160 * 1024, "tile");
+    static_assert(NA >= 1 && NB >= 1 && LDS_BYTES <= 159 * 1024, "tile");
 
     // per_half(k, bv): called with the B fragments of every 32-deep half step (k counts from k0)
     template <typename F>
@@ -251,14 +251,15 @@ static inline unsigned gt_grid(const GtMap& m) { return (unsigned)(((long)m.na *
 // dynamic LDS above 64 KiB has to be asked for, once per kernel and device
 template <auto Kern>
 static int gt_lds(size_t bytes) {
-    if (bytes > 160 * 1024) return -2;
+    constexpr int MOST = 159 * 1024;           // a kilobyte is left for a kernel's static LDS
+    if (bytes > MOST) return -2;
     if (bytes <= 64 * 1024) return 0;
     static std::atomic<unsigned long> done{0};
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return -8;
     const unsigned long bit = 1ul << (dev & 63);
     if (done.load() & bit) return 0;
-    if (hipFuncSetAttribute((const void*)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return -8;
+    if (hipFuncSetAttribute((const void*)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, MOST) != hipSuccess) return -8;
     done.fetch_or(bit);
     return 0;
 }

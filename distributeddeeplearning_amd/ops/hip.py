@@ -2417,9 +2417,25 @@ def _rc(rc, what):
         raise RuntimeError(f"{what}: kernel launch refused (code {rc})")
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
 def _on_device(t):
-    """Launches go to the current device's current stream: make the tensors' device the current one."""
-    return torch.cuda.device(t.device)
+    """Launches go to the current device: make the tensors' device the current one (no cost where it already is)."""
+    return _HERE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+
+
+def _stream_of(t):
+    """The current stream of the tensors' device (the raw handle: torch.cuda.current_stream() builds an object first, 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _chk_out(t, n, dtypes, like, name):
@@ -2487,7 +2503,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
             raise ValueError(f"dense_softmax_ce: N={N} K={K} V={V} outside the kernels' range")
         ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         _rc(_dense_ce(x.data_ptr(), w.data_ptr(), _p(bias), labels.data_ptr(), N, V, K, loss.data_ptr(), rows.data_ptr(),
-                      _p(dx), _p(dw), _p(db), bf, ws.data_ptr(), nws, CE_PIECE_BYTES, CE_TILE, _stream()),
+                      _p(dx), _p(dw), _p(db), bf, ws.data_ptr(), nws, CE_PIECE_BYTES, CE_TILE, _stream_of(x)),
             "dense_softmax_ce")
         _done()
     return loss, dx, dw, db, rows
@@ -2497,7 +2513,9 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
 _pack8 = _sig("ddl_pack8", ci, vp, vp, vp, cl, vp)
 _unpack8 = _sig("ddl_unpack8", ci, vp, vp, vp, cl, vp)
 _act_bwd8 = _sig("ddl_act_bwd8", ci, vp, vp, vp, vp, cl, ci, cf, vp)
-_wgrad8 = _sig("ddl_dense_wgrad8", ci, vp, vp, ci, ci, ci, ci, ci, ci, vp, vp, vp, vp, ci, vp)
+_wgrad8_ws = _sig("ddl_dense_wgrad8_workspace", cl, ci, ci, ci, ci, ci)
+_wgrad8 = _sig("ddl_dense_wgrad8", ci, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, cl, ci, vp)
+WGRAD8_TILE = -1            # tile of dense_wgrad8: -1 = by the sizes (csrc/hip/act8.hip wg8_plan)
 
 
 def _chk_packed(q, name="q"):
@@ -2517,7 +2535,7 @@ def pack8(x):
     scales = torch.empty(ceil_div(x.numel(), 32), dtype=torch.uint8, device=x.device)
     if x.numel():
         with _on_device(x):
-            _rc(_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _stream()), "pack8")
+            _rc(_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _stream_of(x)), "pack8")
             _done()
     return Packed8(codes, scales)
 
@@ -2529,7 +2547,7 @@ def unpack8(q, out=None):
         _chk_out(out, n, (torch.bfloat16,), q.codes, "out")
     if n:
         with _on_device(y):
-            _rc(_unpack8(q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), n, _stream()), "unpack8")
+            _rc(_unpack8(q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), n, _stream_of(y)), "unpack8")
             _done()
     return y
 
@@ -2545,7 +2563,7 @@ def act_bwd8(dy, q, kind, alpha=0.3):
     if n:
         with _on_device(dy):
             _rc(_act_bwd8(dy.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), dx.data_ptr(), n, ACT_CODE[kind], alpha,
-                          _stream()), "act_bwd8")
+                          _stream_of(dy)), "act_bwd8")
             _done()
     return dx
 
@@ -2574,16 +2592,11 @@ def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
             dw.zero_()
             db.zero_()
             return dw, db
-        tile = 0 if ceil_div(K, 256) * ceil_div(O, 256) >= 192 else (1 if ceil_div(K, 128) * ceil_div(O, 128) >= 256 else 2)
-        t = (256, 128, 64)[tile]
-        steps = ceil_div(R, 64)
-        ns = max(1, min((256 if tile == 0 else 512) // (ceil_div(K, t) * ceil_div(O, t)), steps // 4, 64))
-        per = ceil_div(steps, ns) * 64
-        ns = ceil_div(R, per)
-        sw = torch.empty(ns, O, K, dtype=torch.float32, device=dev) if ns > 1 else None
-        sb = torch.empty(ns, O, dtype=torch.float32, device=dev) if ns > 1 else None
-        xh = unpack8(q)
-        _rc(_wgrad8(xh.data_ptr(), dy.data_ptr(), R, K, Op, O, ns, per, dw.data_ptr(), db.data_ptr(), _p(sw), _p(sb), tile,
-                    _stream()), "dense_wgrad8")
+        nws = _wgrad8_ws(R, K, Op, O, WGRAD8_TILE)
+        if nws < 0:
+            raise ValueError(f"dense_wgrad8: R={R} K={K} O={O} of {Op} outside the kernels' range")
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        _rc(_wgrad8(x.data_ptr(), q.scales.data_ptr(), dy.data_ptr(), R, K, Op, O, dw.data_ptr(), db.data_ptr(), _p(ws), nws,
+                    WGRAD8_TILE, _stream_of(dy)), "dense_wgrad8")
         _done()
     return dw, db

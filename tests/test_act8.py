@@ -199,6 +199,24 @@ def test_dense_wgrad8(R, K, Op, O):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
+@pytest.mark.parametrize("R,K,O", [(70, 72, 40), (640, 520, 264), (3000, 136, 72)])
+def test_dense_wgrad8_every_tile(tile, R, K, O, monkeypatch):
+    from distributeddeeplearning_amd.ops import hip
+    monkeypatch.setattr(hip, "WGRAD8_TILE", tile)
+    test_dense_wgrad8(R, K, O, O - 3)
+
+
+@pytest.mark.gpu
+def test_dense_wgrad8_bad_block():
+    """A block that held a NaN or an infinity reads as NaN: its features' gradients, no others."""
+    x, dy = values(130, 64, 1, 0.0), values(130, 16, 2, 0.0)
+    x[77, 5] = math.inf
+    dw, db = F.dense_wgrad8(F.pack8(x.cuda()), dy.cuda())
+    assert torch.isnan(dw[:, :32]).all() and torch.isfinite(dw[:, 32:]).all() and torch.isfinite(db).all()
+
+
+@pytest.mark.gpu
 def test_dense_wgrad8_outputs_streams_and_empty():
     x, dy = values(130, 40, 1, 1.0).cuda(), values(130, 24, 2, 0.0).cuda()
     q = F.pack8(x)
