@@ -686,6 +686,51 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the last fetch has landed before the LDS is given back
 }
 
+// Probabilities of wide rows (prediction): logits [B][Cs] bf16 of which N classes are real -> probs [B][N] fp32.  One block per
+// row: a pass for the running maximum and sum, a second one (the row then comes from L2) for the result; bound by the 4 bytes
+// it writes per class.
+__global__ __launch_bounds__(256) void softmax_wide_kernel(const bf16_t* __restrict__ logits, float* __restrict__ probs, int Cs,
+                                                           int N) {
+    __shared__ float red[4][2];
+    const bf16_t* l = logits + (long)blockIdx.x * Cs;
+    float* o = probs + (long)blockIdx.x * N;
+    const int tid = threadIdx.x;
+    float m = -INFINITY, s = 0.f;
+    auto add = [&](float om, float os) {                      // m = -inf: nothing seen but masked classes (or NaN: s is NaN)
+        const float t = fmaxf(m, om);
+        s = (m == t ? s : s * __expf(m - t)) + (om == t ? os : os * __expf(om - t));
+        m = t;
+    };
+    for (int c = tid * 8; c < N; c += 2048) {                 // Cs is a multiple of 8: the loads stay inside the row
+        float f[8];
+        unpack8(*(const uint4*)(l + c), f);
+        float t = -INFINITY, u = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = c + e < N ? fmaxf(t, f[e]) : t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < N) u += f[e] == -INFINITY ? 0.f : __expf(f[e] - t);
+        add(t, u);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) add(__shfl_xor(m, d, 64), __shfl_xor(s, d, 64));
+    if ((tid & 63) == 0) { red[tid >> 6][0] = m; red[tid >> 6][1] = s; }
+    __syncthreads();
+    m = red[0][0]; s = red[0][1];
+    for (int w = 1; w < 4; ++w) add(red[w][0], red[w][1]);
+    const float inv = 1.f / s;
+    for (int c = tid; c < N; c += 256) {
+        const float f = bf2f(l[c]);
+        o[c] = (f == -INFINITY ? 0.f : __expf(f - m)) * inv;  // every class masked: 0 / 0
+    }
+}
+
+DDL_API int ddl_softmax_wide(const void* logits, float* probs, int B, int Cs, int N, hipStream_t s) {
+    if (B <= 0 || N <= 0 || N > Cs || (Cs & 7)) return -1;
+    softmax_wide_kernel<<<B, 256, 0, s>>>((const bf16_t*)logits, probs, Cs, N);
+    return gt_launched();
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 #define CE_MAX_ROWS 8192      // rows of a piece (their labels are ranked in 32 KiB of LDS)
 

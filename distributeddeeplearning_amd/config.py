@@ -51,6 +51,7 @@ class SearchSpace:
     data_train_size: int = 50000
     batch_size: int = 32                              # Keras fit() default
     channels: int = 3                                 # MNIST stacked x3 (DDL.py:119) or 1
+    keep8: bool = False                               # activations in 8 bits between forward and backward (Network.keep8)
     model_save_directory: str = "./models"
     seed: int = 0
 

@@ -57,6 +57,9 @@ class RandomModel:
             self.net.load_logical_state(keep, strict=False)
         self.opt = FlatOptimizer(self.net, compiled.optimizer)
         self.loss_name = compiled.loss
+        self.net.keep8 = space.keep8
+        if self._wide and self.loss_name != "categorical_crossentropy":
+            raise ValueError(f"{self.net.out_shape[-1]} classes: only categorical_crossentropy has a head that wide")
         self.gen = torch.Generator().manual_seed(seed + 7)
         self.history: List[List[float]] = []
         self.use_graph = (self.device.type == "cuda") if use_graph is None else use_graph
@@ -71,9 +74,16 @@ class RandomModel:
             return F.softmax_mse(logits, y, want_grad, index=index)
         return F.softmax_ce(logits, y, want_grad, index=index)
 
+    @property
+    def _wide(self):
+        """Heads past the fused softmax losses' 64 classes train from class numbers (Network.train_labels)."""
+        return self.net.out_shape[-1] > 64
+
     def _fwd_bwd(self, idx):
         net = self.net
         x = net.prepare_input(self.data.train_x, index=idx)
+        if self._wide:
+            return net.train_labels(x, self.data.train_labels.index_select(0, idx))[0]
         logits = net.forward(x, training=True)
         # the minibatch's labels are read through the same index vector inside the loss kernel (no gather pass)
         loss, dlogits, _ = self._loss(logits, self.data.train_y, index=idx)
@@ -295,7 +305,7 @@ class RandomModel:
 
     # ------------------------------------------------------------------ inference
     def predict(self, x=None, index: Optional[torch.Tensor] = None, batch_size: int = 4096) -> torch.Tensor:
-        """Softmax outputs [N,10] (fp32, on device).  `x` is a resident uint8 image tensor (default:
+        """Softmax outputs [N, classes] (fp32, on device).  `x` is a resident uint8 image tensor (default:
         the training pool) optionally gathered by `index`."""
         x = self.data.train_x if x is None else x
         n = x.shape[0] if index is None else index.numel()
@@ -316,10 +326,12 @@ class RandomModel:
             if idx.numel() == 0:
                 return float("nan")
             pred = self.predict(self.data.train_x, index=idx)
-            target = self.data.train_y.index_select(0, idx)
+            target = (self.data.train_labels if self._wide else self.data.train_y).index_select(0, idx)
         else:
             x, target = validation_data
             pred = self.predict(x)
+        if target.dim() == 1:                       # class numbers
+            return int((pred.argmax(1) == target).sum()) / pred.shape[0]
         correct = F.argmax_match_count(pred, target)
         return int(correct) / pred.shape[0]
 

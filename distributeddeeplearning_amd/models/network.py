@@ -12,7 +12,11 @@ Design (MI355X-first, not a Keras clone):
     friendly reduction dims, odd channel counts of the random search space need no slow path);
     parameters are stored padded the same way and stripped on export;
   * shapes are static so a whole training step can be captured in a hipGraph;
-  * no autograd: every op has a hand-written backward that calls the HIP kernels.
+  * no autograd: every op has a hand-written backward that calls the HIP kernels;
+  * what a training forward keeps for the backward pass is bf16, or with `Network.keep8` 8 bits (ops/functional.py
+    pack8) wherever no fused kernel wants the bf16 tensor;
+  * a softmax head of any width trains and scores from integer labels without its logits (`Network.train_labels`,
+    `Network.score`).
 
 Replaces what Keras' `Model`/`fit` machinery did for the reference (/root/reference/DDL.py:58-96,
 /root/reference/GAN_distributed.py:15-117).
@@ -105,6 +109,11 @@ def _round_up(n, a):
     return (n + a - 1) // a * a
 
 
+def _saved(t):
+    """A tensor kept by the forward pass, out of its 8-bit checkpoint if that is how it was kept."""
+    return F.unpack8(t) if isinstance(t, F.Packed8) else t
+
+
 class _Param:
     """One tensor inside a flat buffer.  `shape` is the physical (padded) shape, `lshape` the
     logical one (same rank): logical data lives in the leading corner, the rest is zero."""
@@ -133,6 +142,12 @@ class Op:
 
     def release(self):
         pass
+
+    def keep8(self, x, y):
+        """After a training forward: keep what the backward pass needs in 8 bits.  `x` / `y` return the op's input and
+        output packed (each packed once, also when two ops keep it).  False: this op's kernels want bf16 -- or the op
+        keeps nothing of its own -- and its output may still be held in bf16."""
+        return False
 
 
 # The streaming 5x5 one-channel weight gradient (ops/hip.py stream1_wgrad) from this many elements of the N-channel
@@ -462,10 +477,16 @@ class ConvOp(Op):
         if self.act not in (None, "linear") and not self.act_bwd_fused:
             if self.dy_premul:
                 self.dy_premul = False
+            elif isinstance(self.y, F.Packed8):
+                dy = F.act_bwd8(dy, self.y, self.act, self.alpha)
             else:
                 dy = F.act_bwd(dy, self.y, self.act, self.alpha)
         x = self.x
         dx = None
+        if isinstance(x, F.Packed8):
+            if self.kind == "dense":
+                return self._bwd_dense8(x, dy, need_dx, need_dw, mul)
+            x = F.unpack8(x) if need_dw else x
         if self.onech == "up" or (self.stream1 and self.stream_used):
             bnd, self.bn_deferred = self.bn_deferred, None
             if need_dw and not need_dx and self.x_affine is None:
@@ -554,6 +575,34 @@ class ConvOp(Op):
             if need_dx and dx is None:
                 dx = F.conv_dgrad(dy, self.w_main if g.depthwise else self.w_alt, g, mul=mul)
         return dx
+
+    def _bwd_dense8(self, q, dy, need_dx, need_dw, mul):
+        """Dense backward, the input kept in 8 bits: the weight gradient reads the codes."""
+        B, shape = q.shape[0], q.shape
+        if need_dw:
+            def wg():
+                bn = self.next_bn       # a bias gradient that is zero by construction or written by the BatchNorm's backward
+                plain = not (bn is not None and ((bn.used_batch_stats and self.act in (None, "linear"))
+                                                 or bn.bias_grad_for is self))
+                F.dense_wgrad8(q.reshape(B, -1), dy.reshape(B, -1), out_dw=self.gkernel, out_db=self.gbias if plain else None,
+                               n_out=self.g.O)
+                if plain:
+                    self._gbias_is_zero = False
+                else:
+                    self._bias_grad(dy)
+            _BR.run(wg, dy)
+        if not need_dx:
+            return None
+        return F.conv_dgrad(dy.reshape(B, 1, 1, -1), self._w4(self.w_alt), self.g, mul=mul).reshape(shape)
+
+    def keep8(self, x, y):
+        if self.onech is not None or self.stream1 or self.in_bn is not None or self.x_affine is not None:
+            return False
+        q = x()
+        if q is not None:
+            self.x = q
+        self.y = y() if self.act not in (None, "linear") and not self.act_bwd_fused else None
+        return True
 
     def _dw_bn_bwd(self, dy, need_dw):
         """Depthwise layer behind a batch-statistics BatchNorm (every `random_layer` of DDL_Normal4.py:52 is followed
@@ -660,11 +709,20 @@ class BNOp(Op):
         self.used_batch_stats, self.groups_used = True, groups
         return scale, shift, mean, invstd
 
+    def keep8(self, x, y):
+        if self.defer_to is not None or self.defer_apply_to is not None:
+            return False                # the neighbour's kernel reads our bf16 input
+        q = x()
+        if q is not None:
+            self.x = q
+        self.y = y() if self.post_act not in (None, "linear") else None
+        return True
+
     def bwd_from_part(self, g, part, part_blocks, need_dw=True):
         """Backward when the consumer already produced g = dL/d(BN output before its activation) together with
         the column sums of (g, g * xhat): finalize + apply only."""
         hip = F.hip_backend()
-        dx, _, _ = hip.bn_bwd(g, self.x, None, self.mean, self.invstd, self.gamma, None, 0.3, True,
+        dx, _, _ = hip.bn_bwd(g, _saved(self.x), None, self.mean, self.invstd, self.gamma, None, 0.3, True,
                               self.prev_act, self.prev_alpha, self.ggamma if need_dw else None,
                               self.gbeta if need_dw else None, None, self.groups_used, part=part,
                               part_blocks=part_blocks)
@@ -674,6 +732,10 @@ class BNOp(Op):
         if self.bwd_done:
             self.bwd_done = False
             return dy
+        if isinstance(self.x, F.Packed8) or isinstance(self.y, F.Packed8):
+            self.x, self.y = _saved(self.x), _saved(self.y)
+        if self.y is None and self.post_act in (None, "linear"):
+            self.y = self.x             # not kept (keep8): nothing behind us to differentiate through it
         conv = self.bias_grad_for
         pre, self.pre_bwd = self.pre_bwd, None
         tgt = self.defer_apply_to
@@ -745,7 +807,13 @@ class ActOp(Op):
         return y
 
     def bwd(self, dy, need_dx=True, need_dw=True):
+        if isinstance(self.y, F.Packed8):
+            return F.act_bwd8(dy, self.y, self.act, self.alpha)
         return F.act_bwd(dy, self.y, self.act, self.alpha)
+
+    def keep8(self, x, y):
+        self.y = y()
+        return True
 
     def release(self):
         self.y = None
@@ -763,6 +831,36 @@ class AffineOp(Op):
         return F.affine(dy, self.scale, 0.0, self.c_true)
 
 
+class _Keep8:
+    """Walks a training forward and hands each op its input and output packed on demand.  A tensor two ops keep (a layer's
+    output is the next one's input, also through reshapes) is packed once; one that an op left in bf16 is not packed for
+    its neighbour on top of that, and neither is the network's input."""
+
+    def __init__(self, x):
+        self.x, self.q, self.held = x, None, True
+
+    def after(self, op, y):
+        if isinstance(op, ViewOp):
+            self.x, self.q = y, None if self.q is None else self.q.reshape(*y.shape)
+            return
+        out = []
+
+        def pack_x():
+            if self.q is None and not self.held:
+                self.q = F.pack8(self.x)
+            return self.q
+
+        def pack_y():
+            if not out:
+                out.append(F.pack8(y))
+            return out[0]
+        kept = op.keep8(pack_x, pack_y)
+        same = y is self.x              # the op passed its input on (a BatchNorm its neighbour applies)
+        self.held = not kept or (same and self.held)
+        self.q = out[0] if out else (self.q if same else None)
+        self.x = y
+
+
 # =============================================================================== network
 class Network:
     def __init__(self, spec: ModelSpec, device="cpu", seed: int = 0, bn_mode: str = "batch"):
@@ -774,6 +872,11 @@ class Network:
         self.bn_mode = bn_mode
         self.softmax_head = False
         self.branch_wgrad = False       # captured steps: wgrad chain as a parallel graph branch (SideBranch)
+        # Keep the activations between forward and backward in 8 bits (33 bytes per 32 elements instead of 64; half a step
+        # of 2^-7 of a block's largest value).  Applies to Dense / Conv2D / Conv2DTranspose / BatchNorm / activation layers
+        # on the general kernels; the input of the network and what the fused one-channel and BatchNorm-on-load kernels read
+        # stay bf16.
+        self.keep8 = False
         # CPU oracle only: round every op's output (forward) and input gradient (backward) to bf16, the points at
         # which the device executor stores bf16 tensors -- the oracle then differs from the device by fp32
         # summation order alone and the end-to-end tests can use tight tolerances (tests/test_layerwise_gpu.py)
@@ -1102,8 +1205,11 @@ class Network:
                 raise ValueError("forward(out=...) needs a final single-channel transposed conv on device")
             last.out_buffer = out
         try:
+            keep = _Keep8(x) if training and self.keep8 else None
             for op in self.ops[start:stop]:
                 x = op.fwd(x, training)
+                if keep is not None:
+                    keep.after(op, x)
                 if self.emulate_bf16 and not self.on_gpu and not isinstance(op, ViewOp) \
                         and not (training and getattr(op, "fp32_handoff", False)):
                     x = x.bfloat16().float()
@@ -1119,8 +1225,10 @@ class Network:
     @staticmethod
     def act_owner(op):
         """(y, act, alpha) if `op` is a conv/dense layer whose activation backward is still a separate
-        pass over dY (not already folded into a following BN), else None."""
-        if isinstance(op, ConvOp) and op.act not in (None, "linear") and not op.act_bwd_fused and op.y is not None:
+        pass over dY (not already folded into a following BN), else None.  A y kept in 8 bits stays with its layer
+        (act_bwd8): the input-gradient kernels multiply by a bf16 tensor."""
+        if (isinstance(op, ConvOp) and op.act not in (None, "linear") and not op.act_bwd_fused and op.y is not None
+                and not isinstance(op.y, F.Packed8)):
             return (op.y, op.act, op.alpha)
         return None
 
@@ -1224,6 +1332,8 @@ class Network:
         for op in self.ops:
             for attr in ("x", "y", "x_img"):
                 t = getattr(op, attr, None)
+                if isinstance(t, F.Packed8):
+                    raise ValueError("narrow_saved: the activations were kept in 8 bits (Network.keep8)")
                 if isinstance(t, torch.Tensor) and t.dim() >= 1:
                     setattr(op, attr, t[lo:hi])
             if isinstance(op, BNOp) and op.mean is not None and op.groups_used > 1:
@@ -1234,6 +1344,40 @@ class Network:
                 op.x_affine = (sc[group].contiguous(), sh[group].contiguous(), 1, ctrue)
             if isinstance(op, ViewOp) and op.in_shape is not None:
                 op.in_shape = (hi - lo,) + tuple(op.in_shape[1:])
+
+    # ------------------------------------------------------------------ softmax head from integer labels
+    def _label_head(self):
+        op = self.ops[-1] if self.ops else None
+        if not (self.softmax_head and isinstance(op, ConvOp) and op.kind == "dense"):
+            raise ValueError("integer labels need a network that ends in a softmax Dense layer")
+        return op
+
+    def _head_in(self, h):
+        return h.reshape(h.shape[0], -1)
+
+    def train_labels(self, x, labels):
+        """Forward and backward of the categorical cross-entropy of a softmax Dense head of any width against class numbers
+        (`labels` int64, negative: sample left out): the head's logits, their gradient and its own weight gradient are
+        one operator that never holds the logits (F.dense_softmax_ce).  Gradients land in `self.G`; returns (mean loss,
+        sample losses).  `x` as prepare_input leaves it."""
+        op = self._label_head()
+        h = self.forward(x, training=True, stop=-1)
+        loss, dh, _, _, rows = F.dense_softmax_ce(self._head_in(h), op.w_main.reshape(op.w_main.shape[0], -1), op.bias, labels,
+                                                  out_dw=op.gkernel, out_db=op.gbias)
+        op._gbias_is_zero = False
+        dh = dh.reshape(h.shape)
+        if self.emulate_bf16 and not self.on_gpu:
+            dh = dh.bfloat16().float()
+        self.backward(dh, start=-1)
+        return loss, rows
+
+    def score(self, x, labels):
+        """(mean loss, sample losses) of a softmax Dense head of any width against class numbers, without gradients."""
+        op = self._label_head()
+        h = self.forward(x, training=False, stop=-1)
+        loss, _, _, _, rows = F.dense_softmax_ce(self._head_in(h), op.w_main.reshape(op.w_main.shape[0], -1), op.bias, labels,
+                                                 want_grad=False)
+        return loss, rows
 
     def predict(self, x, batch_size: int = 4096, prepared: bool = False):
         """Inference forward; applies the softmax of a softmax head (Keras `model.predict`).

@@ -61,6 +61,7 @@ _strip_channels = _sig("ddl_strip_channels", None, vp, vp, cl, ci, ci, vp)
 _spatial_pad = _sig("ddl_spatial_pad", None, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, vp)
 _affine = _sig("ddl_affine", None, vp, vp, cl, ci, ci, cf, cf, vp)
 _softmax_loss = _sig("ddl_softmax_loss", None, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp)
+_softmax_wide = _sig("ddl_softmax_wide", ci, vp, vp, ci, ci, ci, vp)
 _sigmoid_bce = _sig("ddl_sigmoid_bce", None, vp, vp, vp, vp, vp, ci, vp)
 _dense1_blocks = _sig("ddl_dense1_bce_blocks", ci, ci)
 _dense1_bce = _sig("ddl_dense1_bce", ci, vp, vp, vp, cf, cf, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci,
@@ -888,9 +889,16 @@ def _softmax_common(logits, target, mode, want_grad, want_probs=True, n_true=Non
     _chk_act(logits, "logits")
     B, Cs = logits.shape
     N = n_true if target is None else target.shape[1]
-    if N > 64 or N > Cs:
-        raise ValueError("softmax kernels support up to 64 classes")
     dev = logits.device
+    if mode == 0 and 64 < N <= Cs:
+        probs = torch.empty(B, N, dtype=torch.float32, device=dev)
+        if B:
+            with _on_device(logits):
+                _rc(_softmax_wide(logits.data_ptr(), probs.data_ptr(), B, Cs, N, _stream_of(logits)), "softmax")
+        _done()
+        return None, None, probs
+    if N > 64 or N > Cs:
+        raise ValueError("softmax losses support up to 64 classes (wider heads: dense_softmax_ce)")
     probs = torch.empty(B, N, dtype=torch.float32, device=dev) if want_probs else None
     if mode == 0:
         _softmax_loss(logits.data_ptr(), None, None, probs.data_ptr(), None, None, None, B, Cs, N, 0, 0, _stream())
