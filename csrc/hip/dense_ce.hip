@@ -81,13 +81,36 @@ __device__ __forceinline__ void ce_rank(const CeLogitsArgs& a, char* smem, int b
         lab[i] = (unsigned long)l < (unsigned long)a.V ? (int)l : 0x7fffffff;
     }
     __syncthreads();
-    for (int r = r0 + wave; r < min(r0 + CE_RANK_ROWS, a.N); r += NTHR / 64) {
-        const int mine = lab[r];
-        int c = 0;
-        for (int i = lane; i < a.N; i += 64) c += lab[i] < mine || (lab[i] == mine && i < r);
+    constexpr int PER = CE_RANK_ROWS / (NTHR / 64);           // rows of a wave, all compared with a label read once
+    int mine[PER], c[PER];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-        if (lane == 0) a.order[c] = r;
+    for (int q = 0; q < PER; ++q) {
+        mine[q] = lab[min(r0 + wave * PER + q, a.N - 1)];
+        c[q] = 0;
+    }
+    // rows in front of the block's count when their label is not larger, rows behind it when it is smaller (r0 is a multiple
+    // of 32: only the 64 rows around it need the row number itself)
+    const int lo = r0 & ~63, hi = lo + 64;
+    for (int i = lane; i < lo; i += 64) {
+        const int l = lab[i];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) c[q] += l <= mine[q];
+    }
+    if (lo + lane < a.N) {
+        const int i = lo + lane, l = lab[i];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) c[q] += l < mine[q] || (l == mine[q] && i < r0 + wave * PER + q);
+    }
+    for (int i = hi + lane; i < a.N; i += 64) {
+        const int l = lab[i];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) c[q] += l < mine[q];
+    }
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) c[q] += __shfl_xor(c[q], o, 64);
+        if (lane == 0 && r0 + wave * PER + q < a.N) a.order[c[q]] = r0 + wave * PER + q;
     }
 }
 
@@ -347,11 +370,14 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
 }
 
 // ------------------------------------------------------------------------------------------------ 3. label terms
-// Sorted position i starts a class: its rows i, i + 1, .. (ascending) are summed into L[first row] and slot[class] is set
-// to it.  Eight features per thread, 256 threads.  Position n, behind them all, takes the mean of the row losses.
+// Rows in sorted order, in windows of 64 positions: the rows of one class inside a window are a run; its first position i
+// sums it (ascending) into L[i], and next[i] is the window where the class goes on, or -1.  slot[class] is its first run.
+// Windows bound a block's work whatever the labels are (8000 rows, 1000 of them of one class: 340 us with a block per class,
+// 20 so).  Eight features per thread, 256 threads.  Position n, behind them all, takes the mean of the row losses.
+#define CE_RUN 64
 struct CeLabelsArgs {
     const CeRow* row; const int* order; const bf16_t* x; const bf16_t* xs; int N, K;
-    int* slot; float* L; float* Lb;                          // [N][K], [N]
+    int* slot; int* next; float* L; float* Lb;               // [V], [N], [N][K], [N]
     const float* rows_all; const float* count; int n_all; float* loss;      // loss nullptr: not the last piece
 };
 
@@ -360,38 +386,48 @@ __device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chun
         if (a.loss && chunk == 0) ce_mean<256>(a.rows_all, a.count, a.n_all, a.loss);
         return;
     }
-    const int first = a.order[i], lab = a.row[first].label;
-    if (lab < 0 || (i > 0 && a.row[a.order[i - 1]].label == lab)) return;
+    const int lab = a.row[a.order[i]].label;
+    if (lab < 0) return;
+    const bool fresh = i == 0 || a.row[a.order[i - 1]].label != lab;
+    if (!fresh && i % CE_RUN != 0) return;
     const int k = (chunk * 256 + threadIdx.x) * 8, lane = threadIdx.x & 63;
     const bool on = k < a.K;
+    const int end = min((i / CE_RUN + 1) * CE_RUN, a.N);      // of the window
+    const int q = i + lane < end ? a.order[i + lane] : a.order[i];
+    const CeRow c = a.row[q];                                 // a lane per row: the loop's loads do not wait for each other
+    const unsigned long m = __ballot(i + lane < end && c.label == lab);
+    const int n = m == ~0ul ? 64 : __builtin_ctzl(~m);        // the run's rows are the leading lanes
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b = 0.f;
-    for (int p = i; p < a.N; p += 64) {                       // 64 positions at a time; the class ends inside one of them
-        const int q = p + lane < a.N ? a.order[p + lane] : first;
-        const bool same = p + lane < a.N && a.row[q].label == lab;
-        const unsigned long m = __ballot(same);
-        const int n = m == ~0ul ? 64 : __builtin_ctzl(~m);    // sorted: the class's rows are the leading lanes
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-            const int r = __builtin_amdgcn_readlane(q, j);
-            const CeRow c = a.row[r];
-            b += c.rest;
-            if (!on) continue;
-            float xv[8], xr[8];
-            unpack8(*(const uint4*)(a.x + (long)r * a.K + k), xv);
-            unpack8(*(const uint4*)(a.xs + (long)r * a.K + k), xr);
+    constexpr int U = 8;
+    for (int j0 = 0; j0 < n; j0 += U) {                       // U rows' loads in flight, added in row order
+        uint4 xv[U], xr[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += fmaf(c.tg, xv[e], -(c.hi * xr[e]));
+        for (int u = 0; u < U; ++u) {
+            const long r = __builtin_amdgcn_readlane(q, min(j0 + u, n - 1));
+            xv[u] = on ? *(const uint4*)(a.x + r * a.K + k) : make_uint4(0, 0, 0, 0);
+            xr[u] = on ? *(const uint4*)(a.xs + r * a.K + k) : make_uint4(0, 0, 0, 0);
         }
-        if (n < 64) break;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (j0 + u >= n) break;
+            const float tg = __shfl(c.tg, j0 + u, 64), hi = __shfl(c.hi, j0 + u, 64);
+            b += __shfl(c.rest, j0 + u, 64);
+            float fv[8], fr[8];
+            unpack8(xv[u], fv);
+            unpack8(xr[u], fr);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += fmaf(tg, fv[e], -(hi * fr[e]));
+        }
     }
     if (on) {
-        float* o = a.L + (long)first * a.K + k;
+        float* o = a.L + (long)i * a.K + k;
         *(float4*)o = make_float4(s[0], s[1], s[2], s[3]);
         *(float4*)(o + 4) = make_float4(s[4], s[5], s[6], s[7]);
     }
     if (chunk == 0 && threadIdx.x == 0) {
-        a.slot[lab] = first;
-        a.Lb[first] = b;
+        if (fresh) a.slot[lab] = i;
+        a.Lb[i] = b;
+        a.next[i] = end < a.N && a.row[a.order[end]].label == lab ? end : -1;
     }
 }
 __global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) { ce_labels(a, blockIdx.x, blockIdx.y); }
@@ -491,21 +527,38 @@ struct CeDwArgs {
     GtOperand xs, e;                 // column order over the rows: x' [N][K] (columns K), E [N][Vp] (columns Vp)
     int N, V, K;
     const bf16_t* g2; int g2_pitch;  // zero behind row N up to a multiple of 64
-    const int* slot; const float* L; const float* Lb;       // the label terms' remainders (ce_labels)
+    const int* slot; const int* next; const float* L; const float* Lb;      // the label terms' remainders (ce_labels)
     const float* acc_w; const float* acc_b;       // earlier row pieces ([V][K], [V]) or nullptr
     void* dw; void* db; int out_bf16;             // this piece's output: fp32 (possibly the accumulator) or bf16
     // streaming kernel: blocks nv, nv + 1, .. of the first row of the grid finish the splits of dx
     const float* slab; const CeRow* row; const bf16_t* w; bf16_t* dx; int nsplit, nv;
+    // tile kernels: the rows in rsplit pieces of rper (a multiple of 64) when there are few tiles; their partial sums go to
+    // rslab [rsplit][V][K], [rsplit][V] and ce_dw_finish does the rest
+    int rsplit, rper; float* rslab;
     GtMap map;
 };
+
+// what the label terms add to four features / the bias of a class: its runs in order (sl: the first, -1: none)
+__device__ __forceinline__ void ce_label_add(const CeDwArgs& a, int sl, int k, f32x4& d) {
+    for (; sl >= 0; sl = a.next[sl]) {
+        const float4 p = *(const float4*)(a.L + (long)sl * a.K + k);
+        d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
+    }
+}
+__device__ __forceinline__ float ce_label_bias(const CeDwArgs& a, int sl) {
+    float s = 0.f;
+    for (; sl >= 0; sl = a.next[sl]) s += a.Lb[sl];
+    return s;
+}
 
 template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dw_kernel(const CeDwArgs a) {
     using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int ta, tb, one;
-    if (!gt_map(a.map, blockIdx.x, ta, tb, one)) return;
+    int ta, tb, split;
+    if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
     const int k0 = ta * BA, v0 = tb * BB;
+    const int n0 = split * a.rper, n1 = min(n0 + a.rper, a.N);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
     const bool do_db = ta == 0 && wa == 0;                     // wave-uniform
@@ -515,13 +568,13 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int v = v0 + wb * (BB / WB) + 16 * j + fr;
-        slots[j] = v < a.V ? a.slot[v] : -1;
+        slots[j] = v < a.V && !a.rslab ? a.slot[v] : -1;
     }
     // db = E^T g: one more matrix instruction per B fragment j, against a fragment whose rows 4 j and 4 j + 1 are g's two
     // terms and all others zero: one accumulator holds all of them
-    T::run(a.xs, a.e, k0, v0, 0, a.N, smem, acc, [&](int k, const bf16x8_t (&bv)[T::NB]) {
+    T::run(a.xs, a.e, k0, v0, n0, n1, smem, acc, [&](int k, const bf16x8_t (&bv)[T::NB]) {
         if (do_db) {
-            const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + k + 8 * fq);
+            const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + n0 + k + 8 * fq);
             const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < T::NB; ++j) {
@@ -535,14 +588,30 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     // batch-32 case, which is little else than this store, 17 -> 10 us)
     constexpr int PITCH = BA / WA * 2 + 16;
     char* patch = smem + wave * (BB / WB) * PITCH;
+    if (a.rslab) {
+        float* o = a.rslab + (long)split * a.V * a.K;
+        float* ob = a.rslab + (long)a.rsplit * a.V * a.K + (long)split * a.V;
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+            const int v = wv + 16 * j;
+            if (v >= a.V) continue;
+            if (do_db && fq == j) ob[v] = bacc[0] + bacc[1];
+#pragma unroll
+            for (int i = 0; i < T::NA; ++i)
+                if (wk + 16 * i < a.K) *(f32x4*)(o + (long)v * a.K + wk + 16 * i) = acc[i][j];
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int v = wv + 16 * j;
         if (v >= a.V) continue;
-        const int sl = slots[j];
+        for (int sl = slots[j]; __any(sl >= 0); sl = sl >= 0 ? a.next[sl] : -1)       // most 16-class groups have no label
+#pragma unroll
+            for (int i = 0; i < T::NA; ++i)
+                if (sl >= 0 && wk + 16 * i < a.K) acc[i][j] += *(const f32x4*)(a.L + (long)sl * a.K + wk + 16 * i);
         if (do_db && fq == j && a.db) {
-            float b = bacc[0] + bacc[1];
-            if (sl >= 0) b += a.Lb[sl];
+            float b = bacc[0] + bacc[1] + ce_label_bias(a, slots[j]);
             if (a.acc_b) b += a.acc_b[v];
             if (a.out_bf16) ((bf16_t*)a.db)[v] = f2bf(b);
             else ((float*)a.db)[v] = b;
@@ -553,10 +622,6 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
             if (k >= a.K) continue;
             f32x4 d = acc[i][j];
             const long o = (long)v * a.K + k;
-            if (sl >= 0) {
-                const float4 p = *(const float4*)(a.L + (long)sl * a.K + k);
-                d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
-            }
             if (a.acc_w) {
                 const float4 p = *(const float4*)(a.acc_w + o);
                 d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
@@ -573,6 +638,38 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
         const int v = v0 + wb * (BB / WB) + u / CPR, k = k0 + wa * (BA / WA) + u % CPR * 8;
         if (v < a.V && k < a.K)
             *(uint4*)((bf16_t*)a.dw + (long)v * a.K + k) = *(const uint4*)(patch + u / CPR * PITCH + u % CPR * 16);
+    }
+}
+
+// the row splits' partial sums (in split order), the label terms and earlier pieces -> dw, db
+template <bool BF16>
+__global__ __launch_bounds__(256) void ce_dw_finish_kernel(const CeDwArgs a) {
+    const long n = (long)a.V * a.K, t0 = blockIdx.x * 256L + threadIdx.x, stride = gridDim.x * 256L;
+    for (long i = t0 * 4; i < n; i += stride * 4) {
+        const int v = (int)(i / a.K), k = (int)(i - (long)v * a.K);
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        int q = 0;
+        for (; q + 7 < a.rsplit; q += 8) {
+            f32x4 p[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) p[u] = *(const f32x4*)(a.rslab + (q + u) * n + i);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += p[u];
+        }
+        for (; q < a.rsplit; ++q) s += *(const f32x4*)(a.rslab + q * n + i);
+        ce_label_add(a, a.slot[v], k, s);
+        if (a.acc_w) s += *(const f32x4*)(a.acc_w + i);
+        if (BF16) *(uint2*)((bf16_t*)a.dw + i) = make_uint2(pack2bf(s[0], s[1]), pack2bf(s[2], s[3]));
+        else *(f32x4*)((float*)a.dw + i) = s;
+    }
+    if (!a.db) return;
+    for (long v = t0; v < a.V; v += stride) {
+        float s = 0.f;
+        for (int q = 0; q < a.rsplit; ++q) s += a.rslab[a.rsplit * n + (long)q * a.V + v];
+        s += ce_label_bias(a, a.slot[v]);
+        if (a.acc_b) s += a.acc_b[v];
+        if (BF16) ((bf16_t*)a.db)[v] = f2bf(s);
+        else ((float*)a.db)[v] = s;
     }
 }
 
@@ -644,9 +741,7 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
         }
         const int v = wv + 16 * fq + fr;
         if (fq < 2 && v < a.V) {
-            float t = b[0] + b[1];
-            const int sl = fq == 0 ? slots[0] : slots[1];
-            if (sl >= 0) t += a.Lb[sl];
+            float t = b[0] + b[1] + ce_label_bias(a, fq == 0 ? slots[0] : slots[1]);
             if (a.acc_b) t += a.acc_b[v];
             if (BF16) ((bf16_t*)a.db)[v] = f2bf(t);
             else ((float*)a.db)[v] = t;
@@ -679,10 +774,7 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
             for (int i = 0; i < 4; ++i) {
                 const int k = c * KC + 16 * i + 4 * fq;
                 f32x4 d = acc[i][j];
-                if (slots[j] >= 0 && k < a.K) {
-                    const float4 p = *(const float4*)(a.L + (long)slots[j] * a.K + k);
-                    d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
-                }
+                if (k < a.K) ce_label_add(a, slots[j], k, d);
                 if (a.acc_w && v < a.V && k < a.K) {
                     const float4 p = *(const float4*)(a.acc_w + (long)v * a.K + k);
                     d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
@@ -758,8 +850,8 @@ struct CePlan {
     int R;                           // rows per piece
     int Vp, lt, nst, wave_cols;      // logits: tile, stats entries per row, classes per entry
     int xt, ns, per;                 // dx: tile, splits over the classes, classes per split
-    int wt;                          // dw: tile
-    long o_count, o_zt, o_stats, o_row, o_order, o_slot, o_g2, o_xs, o_L, o_Lb, o_E, o_slab, o_accw, o_accb, bytes;
+    int wt, rs, rper;                // dw: tile, splits over the rows, rows per split
+    long o_count, o_zt, o_stats, o_row, o_order, o_slot, o_next, o_g2, o_xs, o_L, o_Lb, o_E, o_slab, o_rslab, o_accw, o_accb, bytes;
     int g2_pitch;
 };
 
@@ -803,18 +895,35 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     }
     // dw: the streaming kernel to 128 rows (100 x 1024 x 20000: 24 us, 128 x 4096 x 50000: 171, where the tiles took 28 and
     // 203; with four steps, 200 x 1024 x 20000: 37 and 37, 256 x 2048 x 50000: 143 and 123)
-    p.wt = p.R <= 128 ? 2 : ((long)ce_cdiv(V, 256) * ce_cdiv(K, 256) >= 256 ? 0 : 1);
-    if (force_tile >= 0 && force_tile / 100 % 10 < 2) p.wt = force_tile / 100 % 10;
-    if (p.wt == 2 && p.R > 64) p.wt = 3;
+    // The tiles by their estimated time as for dx; the rows are split when the tiles are few (8000 rows x 64 x 65 classes, one
+    // tile: 161 us in one piece)
+    {
+        static const int edge[2] = {256, 128}, slots[2] = {256, 512};
+        static const double step_us[2] = {1.75, 1.35}, ends[2] = {5.0, 5.0};
+        const int steps = ce_cdiv(p.R, 64), forced = force_tile >= 0 ? force_tile / 100 % 10 : 9;
+        p.wt = p.R <= 64 ? 2 : 3; p.rs = 1; p.rper = steps * 64;
+        double best = 0;
+        for (int t = 0; t < 2; ++t) {
+            if (forced < 2 ? t != forced : p.R <= 128) continue;
+            const long tiles = (long)ce_cdiv(K, edge[t]) * ce_cdiv(V, edge[t]);
+            for (int want = 1; want <= 32 && (want == 1 || want <= steps / 4); ++want) {
+                const int per = ce_cdiv(steps, want), n = ce_cdiv(steps, per);
+                const double us = (double)ce_cdiv(tiles * n, slots[t]) * (per + ends[t]) * step_us[t] +
+                                  (n > 1 ? 3.0 + 0.15 * n + n * 8.0 * V * K / 4.5e6 : 0.0);
+                if (best == 0 || us < best) { best = us; p.wt = t; p.rs = n; p.rper = per * 64; }
+            }
+        }
+    }
     p.g2_pitch = ce_cdiv(p.R, 64) * 64;
     long o = 0;
     auto take = [&](long bytes) { const long at = o; o += (bytes + 255) / 256 * 256; return at; };
     p.o_count = take(4); p.o_zt = take(4L * p.R); p.o_stats = take(8L * p.R * p.nst);
-    p.o_row = p.o_order = p.o_slot = p.o_g2 = p.o_xs = p.o_L = p.o_Lb = p.o_E = p.o_slab = p.o_accw = p.o_accb = 0;
+    p.o_row = p.o_order = p.o_slot = p.o_next = p.o_g2 = p.o_xs = p.o_L = p.o_Lb = p.o_E = p.o_slab = p.o_rslab = p.o_accw = p.o_accb = 0;
     if (train) {
-        p.o_row = take(32L * p.R); p.o_order = take(4L * p.R); p.o_slot = take(4L * V); p.o_g2 = take(4L * p.g2_pitch);
+        p.o_row = take(32L * p.R); p.o_order = take(4L * p.R); p.o_slot = take(4L * V); p.o_next = take(4L * p.R); p.o_g2 = take(4L * p.g2_pitch);
         p.o_xs = take(2L * p.R * K); p.o_L = take(4L * p.R * K); p.o_Lb = take(4L * p.R); p.o_E = take(2L * p.R * p.Vp);
         if (p.ns > 1) p.o_slab = take(4L * p.ns * p.R * K);
+        if (p.rs > 1) p.o_rslab = take(4L * p.rs * V * (K + 1L));
         if (acc && p.R < N) { p.o_accw = take(4L * V * K); p.o_accb = take(4L * V); }
     }
     p.bytes = o;
@@ -867,8 +976,14 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     const size_t out = (size_t)T::NW * (BB / WB) * (BA / WA * 2 + 16);
     const size_t lds = a.out_bf16 && out > T::LDS_BYTES ? out : T::LDS_BYTES;
     if (int rc = gt_lds<kern>(lds)) return rc;
-    a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, 1, 4);
+    a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, a.rsplit, 4);
     kern<<<gt_grid(a.map), T::NTHR, lds, s>>>(a);
+    if (a.rsplit > 1) {
+        const long nb = ((long)a.V * a.K + 1023) / 1024;
+        const int g = (int)(nb > 2048 ? 2048 : nb);
+        if (a.out_bf16) ce_dw_finish_kernel<true><<<g, 256, 0, s>>>(a);
+        else ce_dw_finish_kernel<false><<<g, 256, 0, s>>>(a);
+    }
     return gt_launched();
 }
 
@@ -945,7 +1060,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         else ce_rows_kernel<true, 256><<<n, 256, 0, s>>>(b);
 
         CeLabelsArgs l;
-        l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot;
+        l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot; l.next = (int*)(ws + p.o_next);
         l.L = (float*)(ws + p.o_L); l.Lb = (float*)(ws + p.o_Lb);
         l.rows_all = rows; l.count = count; l.n_all = N; l.loss = last ? loss : nullptr;
         if (int e = gt_launched()) return e;
@@ -968,8 +1083,10 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
 
         CeDwArgs c;
         c.xs = {xs, K, K}; c.e = {E, p.Vp, p.Vp};
+        c.rsplit = ce_cdiv(n, p.rper); c.rper = p.rper;     // a shorter last piece has fewer splits
+        c.rslab = c.rsplit > 1 ? (float*)(ws + p.o_rslab) : nullptr;
         c.slab = d.slab; c.row = row; c.w = w; c.dx = d.dx; c.nsplit = p.ns; c.nv = 0;
-        c.N = n; c.V = V; c.K = K; c.g2 = g2; c.g2_pitch = p.g2_pitch; c.slot = a.slot; c.L = l.L; c.Lb = l.Lb;
+        c.N = n; c.V = V; c.K = K; c.g2 = g2; c.g2_pitch = p.g2_pitch; c.slot = a.slot; c.next = l.next; c.L = l.L; c.Lb = l.Lb;
         // several pieces add up in fp32: in the output itself, or in the workspace until the last piece rounds
         float* aw = out_bf16 ? (float*)(ws + p.o_accw) : (float*)dw;
         float* ab = out_bf16 ? (float*)(ws + p.o_accb) : (float*)db;

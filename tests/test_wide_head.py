@@ -157,7 +157,7 @@ def cuda(x, w, b, lab):
 
 
 SHAPES = [(1, 8, 1), (1, 16, 65), (2, 24, 1000), (5, 8, 128), (16, 64, 64), (31, 40, 333), (33, 136, 4099), (64, 120, 64),
-          (130, 200, 777), (257, 72, 2051), (300, 520, 515), (513, 264, 769)]
+          (130, 200, 777), (257, 72, 2051), (300, 520, 515), (513, 264, 769), (1100, 64, 65), (2500, 40, 70)]
 
 
 @pytest.mark.gpu
@@ -287,7 +287,7 @@ def test_out_tensors_and_empty_batch(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N,V,classes", [(200, 500, 1), (700, 300, 3), (1500, 4000, 40)])
+@pytest.mark.parametrize("N,V,classes", [(200, 500, 1), (700, 300, 3), (1500, 4000, 40), (3000, 100, 14)])
 def test_many_rows_of_one_class_and_label_terms(N, V, classes):
     """Labels repeat; the label terms are exact, so a class that only its own rows' label terms reach (p ~ 0 elsewhere) has
     its dw row to the output's rounding."""
