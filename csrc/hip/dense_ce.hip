@@ -939,6 +939,7 @@ static int launch_logits(CeLogitsArgs& a, hipStream_t s) {
     constexpr auto kern = ce_logits_kernel<BA, BB, WA, WB, STAGES, STORE>;
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.Vp + BA - 1) / BA, (a.N + BB - 1) / BB, 1, 8);
+    if (!gt_map_ok(a.map)) return -1;
     a.nrank = a.order ? (ce_cdiv(a.N, CE_RANK_ROWS) + 7) / 8 * 8 : 8;
     kern<<<a.nrank + gt_grid(a.map), T::NTHR, lds, s>>>(a);
     return gt_launched();
@@ -960,6 +961,7 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     constexpr auto kern = ce_dx_kernel<BA, BB, WA, WB, STAGES>;
     if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, a.nsplit, 8);
+    if (!gt_map_ok(a.map)) return -1;
     a.nlab_chunks = ce_cdiv(a.K, 2048);
     a.nlab = 0;
     // a launch of its own costs 4 us; in front of the tiles the label blocks hold a tile's LDS, so only while they are few
@@ -977,6 +979,7 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     const size_t lds = a.out_bf16 && out > T::LDS_BYTES ? out : T::LDS_BYTES;
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, a.rsplit, 4);
+    if (!gt_map_ok(a.map)) return -1;
     kern<<<gt_grid(a.map), T::NTHR, lds, s>>>(a);
     if (a.rsplit > 1) {
         const long nb = ((long)a.V * a.K + 1023) / 1024;

@@ -247,6 +247,7 @@ static inline GtMap gt_make_map(int na, int nb, int ns, int gb) {
     return m;
 }
 static inline unsigned gt_grid(const GtMap& m) { return (unsigned)(((long)m.na * m.nb * m.ns + 7) / 8 * 8); }
+static inline bool gt_map_ok(const GtMap& m) { return (long)m.na * m.nb * m.ns < (1L << 30); }      // gt_map counts in int
 
 // dynamic LDS above 64 KiB has to be asked for, once per kernel and device
 template <auto Kern>

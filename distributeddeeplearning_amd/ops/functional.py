@@ -312,14 +312,21 @@ def unpack8(q, out=None):
     return (hip_backend() if q.codes.is_cuda else cpu_ref).unpack8(q, out)
 
 
+def _same_device(dy, q):
+    if dy.device != q.codes.device or q.scales.device != q.codes.device:
+        raise ValueError(f"dy is on {dy.device}, the checkpoint's codes on {q.codes.device}, its scales on {q.scales.device}")
+
+
 def act_bwd8(dy, q, kind, alpha=0.3):
     """Activation backward dx = dy * act'(y) with y = act(x) read from its 8-bit checkpoint."""
+    _same_device(dy, q)
     return _b(dy).act_bwd8(dy, q, kind, alpha)
 
 
 def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
     """Gradients of a Dense layer's weights [O][K] and bias [O] (fp32) from its input's 8-bit checkpoint [R][K] and
     dy [R][Op]; `n_out`: O, when dy carries padding lanes behind it."""
+    _same_device(dy, q)
     return _b(dy).dense_wgrad8(q, dy, out_dw, out_db, n_out)
 
 

@@ -11,6 +11,7 @@ Device tensor convention: bf16, channel (last) dim padded to a multiple of 8, pa
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from pathlib import Path
 from typing import Dict, Optional, Tuple
@@ -2410,7 +2411,7 @@ def conv_wgrad(x, dy, g: ConvGeom, layout="A", out=None, box=None, x_affine=None
 
 
 # ------------------------------------------------------------------------------ wide softmax head
-_dense_ce_ws = _sig("ddl_dense_ce_workspace", cl, ci, ci, ci, ci, ci, cl, ci)
+_dense_ce_ws = functools.lru_cache(maxsize=4096)(_sig("ddl_dense_ce_workspace", cl, ci, ci, ci, ci, ci, cl, ci))
 _dense_ce = _sig("ddl_dense_ce", ci, vp, vp, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp, ci, vp, cl, cl, ci, vp)
 
 # Bound on the exponentials a training call keeps at a time, 2 bytes per row and class; a batch that needs more goes
@@ -2521,7 +2522,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
 _pack8 = _sig("ddl_pack8", ci, vp, vp, vp, cl, vp)
 _unpack8 = _sig("ddl_unpack8", ci, vp, vp, vp, cl, vp)
 _act_bwd8 = _sig("ddl_act_bwd8", ci, vp, vp, vp, vp, cl, ci, cf, vp)
-_wgrad8_ws = _sig("ddl_dense_wgrad8_workspace", cl, ci, ci, ci, ci, ci)
+_wgrad8_ws = functools.lru_cache(maxsize=4096)(_sig("ddl_dense_wgrad8_workspace", cl, ci, ci, ci, ci, ci))
 _wgrad8 = _sig("ddl_dense_wgrad8", ci, vp, vp, vp, ci, ci, ci, ci, vp, vp, vp, cl, ci, vp)
 WGRAD8_TILE = -1            # tile of dense_wgrad8: -1 = by the sizes (csrc/hip/act8.hip wg8_plan)
 

@@ -235,6 +235,20 @@ def test_dense_wgrad8_outputs_streams_and_empty():
 
 
 @pytest.mark.gpu
+def test_more_than_2_to_31_elements():
+    n = (1 << 31) + 8 * 40
+    x = torch.empty(n // 8, 8, dtype=torch.bfloat16, device="cuda").normal_()
+    q = F.pack8(x)
+    y = F.unpack8(q)
+    d = F.act_bwd8(x, q, "relu")
+    for rows in (slice(0, 512), slice((1 << 28) - 256, None)):       # around the start and past 2^31 elements
+        part = x[rows].cpu()
+        ref = F.unpack8(F.pack8(part.float()))
+        assert torch.equal(y[rows].float().cpu(), ref)
+        assert torch.equal(d[rows].cpu(), torch.where(part > 0, part, torch.zeros_like(part)))
+
+
+@pytest.mark.gpu
 def test_captured_checkpoint_round_trip():
     from distributeddeeplearning_amd.utils import hipgraph
     x, dy = values(70, 72, 1, 1.0).cuda(), values(70, 72, 2, 0.0).cuda()
@@ -266,6 +280,7 @@ def test_refusals():
                  lambda: F.dense_wgrad8(q, x, out_db=torch.empty(31, device="cuda")),
                  lambda: F.unpack8(q, out=torch.empty(8, 32, device="cuda")),
                  lambda: F.unpack8(F.Packed8(q.codes.t(), q.scales)),
-                 lambda: F.dense_wgrad8(q.reshape(2, 4, 32), x)):
+                 lambda: F.dense_wgrad8(q.reshape(2, 4, 32), x), lambda: F.act_bwd8(x.cpu(), q, "relu"),
+                 lambda: F.dense_wgrad8(q, x.cpu())):
         with pytest.raises(ValueError):
             call()

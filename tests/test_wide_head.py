@@ -273,6 +273,40 @@ def test_row_pieces(N, dtype, monkeypatch):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits(monkeypatch):
+    """8192 rows x 270001 classes in one piece: the exponentials end 4.4 GB behind their start."""
+    from distributeddeeplearning_amd.ops import hip
+    monkeypatch.setattr(hip, "CE_PIECE_BYTES", 8 << 30)
+    N, K, V = 8192, 64, 270001
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(N, K, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(V, K, generator=g, device="cuda") / 8).bfloat16()
+    b = torch.randn(V, generator=g, device="cuda") * 0.1
+    lab = torch.randint(0, V, (N,), generator=g, device="cuda")
+    lab[-1] = V - 1
+    loss, dx, dw, db, rows = F.dense_softmax_ce(x, w, b, lab)
+    lse = torch.empty(N, dtype=torch.float64, device="cuda")
+    p_last = torch.empty(N, 8, dtype=torch.float64, device="cuda")          # the last eight classes' gradients
+    for r in range(0, N, 1024):
+        z = x[r:r + 1024].double() @ w.double().t() + b.double()
+        lse[r:r + 1024] = torch.logsumexp(z, 1)
+        p_last[r:r + 1024] = torch.exp(z[:, -8:] - lse[r:r + 1024, None])
+    zt = (x.double() * w[lab].double()).sum(1) + b[lab].double()
+    assert ((rows.double() - (lse - zt)).abs() <= 2.0 ** -18 * (1 + lse.abs() + zt.abs())).all()
+    p_last -= torch.nn.functional.one_hot((lab - (V - 8)).clamp_min(-1) + 1, 9)[:, 1:].double()
+    p_last /= N
+    ref = p_last.t() @ x.double()
+    lim = 2 * U16 * 1.01 * (p_last.abs().t() @ x.double().abs()) + 1e-9
+    assert ((dw[-8:].double() - ref).abs() <= lim).all()
+    assert ((db[-8:].double() - p_last.sum(0)).abs() <= 1.01 * U16 * p_last.abs().sum(0) + 1e-9).all()
+    last = slice(N - 4, N)
+    p = torch.exp(x[last].double() @ w.double().t() + b.double() - lse[last, None])
+    p[torch.arange(4, device="cuda"), lab[last]] -= 1
+    ref = p @ w.double() / N
+    assert ((dx[last].double() - ref).abs() <= 1.01 * (U16 * (p.abs() @ w.double().abs()) / N + U16 * ref.abs())).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_out_tensors_and_empty_batch(dtype):
     a = make(20, 40, 130, seed=2)
