@@ -32,6 +32,8 @@
 
 #define CE_LOG2E 1.44269504088896340736f
 #define CE_LN2 0.69314718055994530942f
+constexpr long CE_CACHE = 256L << 20;      // the last level cache, shared by the whole chip
+constexpr int CE_NT = 2;                   // a raw buffer store's policy: non-temporal
 
 // What the later kernels need of a row: the gradient of its logits is g E, plus `rest` in the label's class.
 struct CeRow { float g, hi, tg, rest; int label; int pad[3]; };      // hi = E[label], tg = dl[label], rest = tg - hi g
@@ -551,9 +553,9 @@ __device__ __forceinline__ float ce_label_bias(const CeDwArgs& a, int sl) {
     return s;
 }
 
-template <int BA, int BB, int WA, int WB, int STAGES>
+template <int BA, int BB, int WA, int WB, int STAGES, int BK>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dw_kernel(const CeDwArgs a) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO, BK>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int ta, tb, split;
     if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
@@ -584,8 +586,9 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
         }
     });
     const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
-    // bf16 rows leave through the wave's own LDS patch as whole 16-byte groups (8-byte stores of 16 rows at a time: the
-    // batch-32 case, which is little else than this store, 17 -> 10 us)
+    // bf16 rows leave through the wave's own LDS patch as whole 16-byte groups (8-byte stores of 16 rows at a time: 17 -> 10
+    // us of a batch of 32), past the caches: the next reader is the optimiser (the whole step of 1237 x 776 x 30011: 281 ->
+    // 270 us, of 96 x 2048 x 60000 256 -> 224, of 512 x 1024 x 50021 228 -> 231)
     constexpr int PITCH = BA / WA * 2 + 16;
     char* patch = smem + wave * (BB / WB) * PITCH;
     if (a.rslab) {
@@ -637,7 +640,8 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     for (int u = lane; u < (BB / WB) * CPR; u += 64) {
         const int v = v0 + wb * (BB / WB) + u / CPR, k = k0 + wa * (BA / WA) + u % CPR * 8;
         if (v < a.V && k < a.K)
-            *(uint4*)((bf16_t*)a.dw + (long)v * a.K + k) = *(const uint4*)(patch + u / CPR * PITCH + u % CPR * 16);
+            __builtin_nontemporal_store(*(const gt_u32x4*)(patch + u / CPR * PITCH + u % CPR * 16),
+                                        (gt_u32x4*)((bf16_t*)a.dw + (long)v * a.K + k));
     }
 }
 
@@ -791,7 +795,7 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
             const int u = t * 64 + lane, row = u / CPR, g = u % CPR;
             const int k = c * KC + g * (16 / ES);
             const unsigned off = (wv + row < a.V && k < a.K) ? (unsigned)(((wave * WV + row) * a.K + k) * ES) : GT_OOB;
-            __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t*)(patch + row * PITCH + g * 16), rs, off, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4_t*)(patch + row * PITCH + g * 16), rs, off, 0, CE_NT);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the last fetch has landed before the LDS is given back
@@ -895,11 +899,14 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     }
     // dw: the streaming kernel to 128 rows (100 x 1024 x 20000: 24 us, 128 x 4096 x 50000: 171, where the tiles took 28 and
     // 203; with four steps, 200 x 1024 x 20000: 37 and 37, 256 x 2048 x 50000: 143 and 123)
-    // The tiles by their estimated time as for dx; the rows are split when the tiles are few (8000 rows x 64 x 65 classes, one
-    // tile: 161 us in one piece)
+    // The tiles by their estimated time: a CU holds one 256 x 256 block or three of 128 x 128, which are out of step with one
+    // another, so one's store runs under the others' products (stages of 32 rows: three blocks' LDS fits.  512 x 1024 x 50021:
+    // 82 us, 256 x 256 tiles 96; 256 x 2048 x 50000: 110 and 132; 4096 x 2048 x 32768: 618 and 555; 8192 x 4096 x 131072: 10.8
+    // and 7.4 ms.  Two blocks with stages of 64 rows took 106 on the first, two of 256 x 128 88).  The rows are split when the
+    // tiles are few (8000 rows x 64 x 65 classes, one tile: 161 us in one piece)
     {
-        static const int edge[2] = {256, 128}, slots[2] = {256, 512};
-        static const double step_us[2] = {1.75, 1.35}, ends[2] = {5.0, 5.0};
+        static const int edge[2] = {256, 128}, fit[2] = {1, 3};
+        static const double round_us[2] = {1.75, 1.64}, one_us[2] = {1.75, 1.3}, ends[2] = {8.0, 3.5};
         const int steps = ce_cdiv(p.R, 64), forced = force_tile >= 0 ? force_tile / 100 % 10 : 9;
         p.wt = p.R <= 64 ? 2 : 3; p.rs = 1; p.rper = steps * 64;
         double best = 0;
@@ -908,7 +915,8 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
             const long tiles = (long)ce_cdiv(K, edge[t]) * ce_cdiv(V, edge[t]);
             for (int want = 1; want <= 32 && (want == 1 || want <= steps / 4); ++want) {
                 const int per = ce_cdiv(steps, want), n = ce_cdiv(steps, per);
-                const double us = (double)ce_cdiv(tiles * n, slots[t]) * (per + ends[t]) * step_us[t] +
+                const double share = (double)ce_cdiv(tiles * n, 256) / fit[t] * round_us[t];
+                const double us = (share > one_us[t] ? share : one_us[t]) * (per + ends[t]) +
                                   (n > 1 ? 3.0 + 0.15 * n + n * 8.0 * V * K / 4.5e6 : 0.0);
                 if (best == 0 || us < best) { best = us; p.wt = t; p.rs = n; p.rper = per * 64; }
             }
@@ -971,10 +979,10 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     return gt_launched();
 }
 
-template <int BA, int BB, int WA, int WB, int STAGES>
+template <int BA, int BB, int WA, int WB, int STAGES, int BK>
 static int launch_dw(CeDwArgs& a, hipStream_t s) {
-    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO>;
-    constexpr auto kern = ce_dw_kernel<BA, BB, WA, WB, STAGES>;
+    using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO, BK>;
+    constexpr auto kern = ce_dw_kernel<BA, BB, WA, WB, STAGES, BK>;
     const size_t out = (size_t)T::NW * (BB / WB) * (BA / WA * 2 + 16);
     const size_t lds = a.out_bf16 && out > T::LDS_BYTES ? out : T::LDS_BYTES;
     if (int rc = gt_lds<kern>(lds)) return rc;
@@ -1031,11 +1039,15 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
     bf16_t* E = (bf16_t*)(ws + p.o_E);
     bf16_t* xs = (bf16_t*)(ws + p.o_xs);
     bf16_t* g2 = (bf16_t*)(ws + p.o_g2);
+    // The weights are read past the caches where one row tile is all there is and nobody reads them again soon: when scoring
+    // (32 x 2048 x 65536: 67 -> 60 us) and in a step whose dx would not find them there either (32 x 4096 x 100000: 642 -> 575
+    // us; 64 x 2048 x 30000, whose weights stay: 116 -> 124, so there not)
+    static const int l_rows[4] = {256, 128, 32, 32}, x_rows[3] = {256, 128, 32};
     for (int r0 = 0; r0 < N; r0 += p.R) {
         const int n = N - r0 < p.R ? N - r0 : p.R;
         const bool last = r0 + n >= N;
         CeLogitsArgs a;
-        a.w = {w, K, V}; a.x = {x + (long)r0 * K, K, n};
+        a.w = {w, K, V, n <= l_rows[p.lt] && (!train || 2L * V * K > CE_CACHE)}; a.x = {x + (long)r0 * K, K, n};
         a.bias = bias; a.labels = labels + r0; a.N = n; a.V = V; a.K = K; a.Vp = p.Vp;
         a.E = train ? E : nullptr; a.stats = (float2*)(ws + p.o_stats); a.nst = p.nst; a.zt = zt;
         a.labels_all = labels; a.n_all = N; a.count = r0 == 0 ? count : nullptr;
@@ -1070,7 +1082,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
 
         CeDxArgs d;
         d.lab = l;
-        d.w = {w, K, K}; d.e = {E, p.Vp, n};
+        d.w = {w, K, K, n <= x_rows[p.xt] && 2L * V * K > CE_CACHE}; d.e = {E, p.Vp, n};
         d.N = n; d.V = V; d.K = K; d.nsplit = p.ns; d.per_split = p.per; d.row = row; d.dx = (bf16_t*)dx + (long)r0 * K;
         d.slab = p.ns > 1 ? (float*)(ws + p.o_slab) : nullptr;
         switch (p.xt) {
@@ -1099,8 +1111,8 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         c.dw = last ? dw : (void*)aw;
         c.db = db ? (last ? db : (void*)ab) : nullptr;
         switch (p.wt) {
-            case 0: rc = launch_dw<256, 256, 2, 4, 2>(c, s); break;
-            case 1: rc = launch_dw<128, 128, 2, 2, 2>(c, s); break;
+            case 0: rc = launch_dw<256, 256, 2, 4, 2, 64>(c, s); break;
+            case 1: rc = launch_dw<128, 128, 2, 2, 3, 32>(c, s); break;
             case 2: rc = c.out_bf16 ? launch_dw_thin<true, 1>(c, s) : launch_dw_thin<false, 1>(c, s); break;
             default: rc = c.out_bf16 ? launch_dw_thin<true, 2>(c, s) : launch_dw_thin<false, 2>(c, s);
         }

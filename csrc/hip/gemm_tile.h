@@ -12,7 +12,8 @@
 //   column order: the four k rows a 16-lane group transposes, times the two groups of a 32-lane half, are eight rows
 //                 whose 32-byte units must fall into eight different units of the 256-byte bank row: unit ^ f(k row)
 // Rows, columns and k groups beyond the operand fetch an out-of-range offset, which writes zeros.
-// One barrier per 64-deep step; the DMA of the next STAGES - 1 steps is in flight across it, retired by a counted vmcnt.
+// One barrier per step (64 deep; 32 where both operands come in column order and more blocks are to fit a CU); the DMA
+// of the next STAGES - 1 steps is in flight across it, retired by a counted vmcnt.
 // The DMA is inline asm because behind the builtin the compiler drains vmcnt in front of every transposing LDS read
 // (it cannot tell it from a reader of the buffer in flight); it has no register output, only LDS, and every wait for
 // it is the explicit one in front of the barrier.
@@ -31,6 +32,13 @@ __device__ __forceinline__ void gt_dma16(gt_u32x4 rs, unsigned voff, unsigned ld
                  : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_base));
 }
 
+// the same for memory that nobody reads again soon: non-temporal, it displaces nothing
+__device__ __forceinline__ void gt_dma16_once(gt_u32x4 rs, unsigned voff, unsigned lds_base) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_base));
+}
+
 __device__ __forceinline__ s16x4 gt_tr_read(const char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(p));
 }
@@ -38,19 +46,22 @@ __device__ __forceinline__ s16x4 gt_tr_read(const char* p) {
 // One operand of a tile: `p` the tensor, `ld` elements per memory row.  Row order: rows [0, n) of length >= k_end.
 // Column order: k rows [0, k_end) of which columns [0, n) are real.  n and ld are multiples of 8 in column order, k_end
 // and ld in row order (16-byte groups are all in or all out).
+// once: operand A is read by one tile only and not wanted in the caches (tiles of at most 128 in b; the others ignore it)
 struct GtOperand {
     const bf16_t* p;
     long ld;
     int n;
+    bool once = false;
 };
 
-// TR = column order.  T rows (columns) per tile, NW waves in the block.
-template <int T, int NW, bool TR>
+// TR = column order.  T rows (columns) per tile, NW waves in the block, BK the depth of a stage.
+template <int T, int NW, bool TR, int BK = GT_BK>
 struct GtStage {
-    static constexpr int PIECES = T / 8;                              // 1-KiB pieces per stage
+    static_assert(TR || BK == 64, "row order: 128-byte LDS rows");
+    static constexpr int PIECES = T * BK / 512;                       // 1-KiB pieces per stage
     static constexpr int P = (PIECES + NW - 1) / NW;                  // per wave (fewer pieces than waves: some are
     static_assert(PIECES % NW == 0 || NW % PIECES == 0, "tile");      //  fetched twice, so every wave counts alike)
-    static constexpr int BYTES = T * GT_BK * 2;
+    static constexpr int BYTES = T * BK * 2;
     static constexpr int SLOTS = TR ? T / 8 : 8;                      // 16-byte slots per LDS row
     static constexpr int RPP = 64 / SLOTS;                            // LDS rows per piece
 
@@ -86,10 +97,11 @@ struct GtStage {
             }
         }
         base = (unsigned long)o.p + (TR ? (long)k0 * ld2 + (long)t0 * 2 : (long)t0 * ld2 + (long)k0 * 2);
-        step_bytes = TR ? GT_BK * ld2 : GT_BK * 2;
+        step_bytes = TR ? BK * ld2 : BK * 2;
     }
 
     // DMA of the next step into LDS at byte address `lds` (uniform); steps past the end write zeros
+    template <bool ONCE = false>
     __device__ __forceinline__ void issue(unsigned lds, int wave) {
         unsigned num = 0x7FFFFFF0u;
         if (TR) {                       // k rows past the end lie beyond the descriptor
@@ -105,10 +117,11 @@ struct GtStage {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int piece = PIECES >= NW ? wave * P + i : wave % PIECES;
-            gt_dma16(rs, in ? voff[i] : GT_OOB, lds + piece * 1024);
+            if (ONCE) gt_dma16_once(rs, in ? voff[i] : GT_OOB, lds + piece * 1024);
+            else gt_dma16(rs, in ? voff[i] : GT_OOB, lds + piece * 1024);
         }
         base += step_bytes;
-        left -= GT_BK;
+        left -= BK;
     }
 };
 
@@ -150,12 +163,12 @@ struct GtFrag {
 //   2 scheduling fence   1184  1306  1200
 enum GtSched { GT_PLAIN = 0, GT_PRIO = 1, GT_FENCE = 2 };
 
-template <int BA, int BB, int WA, int WB, bool TA, bool TB, int STAGES, int SCHED>
+template <int BA, int BB, int WA, int WB, bool TA, bool TB, int STAGES, int SCHED, int BK = GT_BK>
 struct GtTile {
     static constexpr int NW = WA * WB, NTHR = 64 * NW;
     static constexpr int NA = BA / WA / 16, NB = BB / WB / 16;
-    using SA = GtStage<BA, NW, TA>;
-    using SB = GtStage<BB, NW, TB>;
+    using SA = GtStage<BA, NW, TA, BK>;
+    using SB = GtStage<BB, NW, TB, BK>;
     static constexpr int STAGE_BYTES = SA::BYTES + SB::BYTES;
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
     static constexpr int P = SA::P + SB::P;
@@ -164,6 +177,13 @@ struct GtTile {
     // per_half(k, bv): called with the B fragments of every 32-deep half step (k counts from k0)
     template <typename F>
     static __device__ __forceinline__ void run(const GtOperand& A, const GtOperand& B, int a0, int b0, int k0, int k1,
+                                               char* smem, f32x4 (&acc)[NA][NB], F&& per_half) {
+        if (BB <= 128 && A.once) run_as<true>(A, B, a0, b0, k0, k1, smem, acc, per_half);
+        else run_as<false>(A, B, a0, b0, k0, k1, smem, acc, per_half);
+    }
+    // two loops: a branch at every issue cost the tiles of 128 rows 2 %
+    template <bool ONCE, typename F>
+    static __device__ __forceinline__ void run_as(const GtOperand& A, const GtOperand& B, int a0, int b0, int k0, int k1,
                                                char* smem, f32x4 (&acc)[NA][NB], F&& per_half) {
         const int lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -180,10 +200,10 @@ struct GtTile {
 #pragma unroll
             for (int j = 0; j < NB; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-        const int nsteps = (k1 - k0 + GT_BK - 1) / GT_BK;
+        const int nsteps = (k1 - k0 + BK - 1) / BK;
 #pragma unroll
         for (int d = 0; d < STAGES - 1; ++d) {
-            sa.issue(lds0 + d * STAGE_BYTES, wave);
+            sa.template issue<ONCE>(lds0 + d * STAGE_BYTES, wave);
             sb.issue(lds0 + d * STAGE_BYTES + SA::BYTES, wave);
         }
         int cur = 0, nxt = STAGES - 1;
@@ -193,11 +213,11 @@ struct GtTile {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * P) : "memory");
             // A's DMA here, B's between the half steps: issued together (eight instructions on a full queue) they held up
             // the first fragment reads of the step; 4 - 9 % on all three products
-            sa.issue(lds0 + nxt * STAGE_BYTES, wave);
+            sa.template issue<ONCE>(lds0 + nxt * STAGE_BYTES, wave);
             const char* ta = smem + cur * STAGE_BYTES;
             const char* tb = ta + SA::BYTES;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
+            for (int kk = 0; kk < BK / 32; ++kk) {
                 bf16x8_t av[NA], bv[NB];
 #pragma unroll
                 for (int i = 0; i < NA; ++i) av[i] = fa.load(ta, i, kk, wa * (BA / WA / 16));
@@ -211,7 +231,7 @@ struct GtTile {
                     for (int i = 0; i < NA; ++i)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[i], bv[j], acc[i][j], 0, 0, 0);
                 if (SCHED == GT_PRIO) __builtin_amdgcn_s_setprio(0);
-                per_half(s * GT_BK + kk * 32, bv);
+                per_half(s * BK + kk * 32, bv);
                 if (kk == 0) sb.issue(lds0 + nxt * STAGE_BYTES + SA::BYTES, wave);
             }
             if (++cur == STAGES) cur = 0;
