@@ -440,7 +440,7 @@ struct CeDxArgs {
     int N, V, K;
     int nsplit, per_split;           // classes per split (a multiple of 64)
     const CeRow* row; bf16_t* dx; float* slab;    // slab [nsplit][N][K] when nsplit > 1
-    CeLabelsArgs lab; int nlab, nlab_chunks;      // few rows: the first nlab blocks (a multiple of 8) do the label terms
+    CeLabelsArgs lab; int ntile, nlab_chunks;     // blocks of 256 threads behind the ntile of the tiles do the label terms
     GtMap map;
 };
 
@@ -462,13 +462,13 @@ template <int BA, int BB, int WA, int WB, int STAGES>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dx_kernel(const CeDxArgs a) {
     using T = GtTile<BA, BB, WA, WB, true, false, STAGES, GT_FENCE>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    if (T::NTHR == 256 && (int)blockIdx.x < a.nlab) {
-        const int i = blockIdx.x / a.nlab_chunks;
-        if (i <= a.lab.N) ce_labels(a.lab, i, blockIdx.x - i * a.nlab_chunks);
+    if (T::NTHR == 256 && (int)blockIdx.x >= a.ntile) {
+        const int b = blockIdx.x - a.ntile, i = b / a.nlab_chunks;
+        ce_labels(a.lab, i, b - i * a.nlab_chunks);
         return;
     }
     int ta, tb, split;
-    if (!gt_map(a.map, blockIdx.x - a.nlab, ta, tb, split)) return;
+    if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
     const int k0 = ta * BA, r0 = tb * BB;
     const int v0 = split * a.per_split, v1 = min(v0 + a.per_split, a.V);
     f32x4 acc[T::NA][T::NB];
@@ -532,7 +532,7 @@ struct CeDwArgs {
     const int* slot; const int* next; const float* L; const float* Lb;      // the label terms' remainders (ce_labels)
     const float* acc_w; const float* acc_b;       // earlier row pieces ([V][K], [V]) or nullptr
     void* dw; void* db; int out_bf16;             // this piece's output: fp32 (possibly the accumulator) or bf16
-    // streaming kernel: blocks nv, nv + 1, .. of the first row of the grid finish the splits of dx
+    // blocks nv, nv + 1, .. (of the first row of the grid; of 256 threads) finish the splits of dx
     const float* slab; const CeRow* row; const bf16_t* w; bf16_t* dx; int nsplit, nv;
     // tile kernels: the rows in rsplit pieces of rper (a multiple of 64) when there are few tiles; their partial sums go to
     // rslab [rsplit][V][K], [rsplit][V] and ce_dw_finish does the rest
@@ -557,6 +557,10 @@ template <int BA, int BB, int WA, int WB, int STAGES, int BK>
 __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dw_kernel(const CeDwArgs a) {
     using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO, BK>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    if (T::NTHR == 256 && (int)blockIdx.x >= a.nv) {
+        ce_dx_finish(a.slab, a.row, a.w, a.dx, a.N, a.K, a.nsplit, blockIdx.x - a.nv, gridDim.x - a.nv);
+        return;
+    }
     int ta, tb, split;
     if (!gt_map(a.map, blockIdx.x, ta, tb, split)) return;
     const int k0 = ta * BA, v0 = tb * BB;
@@ -971,11 +975,13 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, a.nsplit, 8);
     if (!gt_map_ok(a.map)) return -1;
     a.nlab_chunks = ce_cdiv(a.K, 2048);
-    a.nlab = 0;
-    // a launch of its own costs 4 us; in front of the tiles the label blocks hold a tile's LDS, so only while they are few
-    if (a.N <= 128 && T::NTHR == 256) a.nlab = (a.nlab_chunks * (a.N + 1) + 7) / 8 * 8;
-    else ce_labels_kernel<<<dim3(a.N + 1, a.nlab_chunks), 256, 0, s>>>(a.lab);
-    kern<<<a.nlab + gt_grid(a.map), T::NTHR, T::LDS_BYTES, s>>>(a);
+    a.ntile = gt_grid(a.map);
+    // The label blocks fill what the last round of tiles leaves (a launch of their own costs 5 us; the large tiles have other
+    // blocks and do not notice).  They hold a tile's LDS, so not when they are many (8000 x 64 x 65: 162 us, 125 on their own)
+    const int nlab = a.nlab_chunks * (a.N + 1);
+    const bool ride = T::NTHR == 256 && nlab <= 2048;
+    if (!ride) ce_labels_kernel<<<dim3(a.N + 1, a.nlab_chunks), 256, 0, s>>>(a.lab);
+    kern<<<a.ntile + (ride ? nlab : 0), T::NTHR, T::LDS_BYTES, s>>>(a);
     return gt_launched();
 }
 
@@ -988,7 +994,11 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, a.rsplit, 4);
     if (!gt_map_ok(a.map)) return -1;
-    kern<<<gt_grid(a.map), T::NTHR, lds, s>>>(a);
+    // the splits of dx are finished in what the last round of tiles leaves, or by a launch of their own (7 us)
+    a.nv = gt_grid(a.map);
+    const int nfin = a.slab ? (int)(((long)a.N * a.K + 1023) / 1024) : 0;
+    if (T::NTHR != 256 && nfin) ce_dx_finish_kernel<<<nfin, 256, 0, s>>>(a.slab, a.row, a.w, a.dx, a.N, a.K, a.nsplit);
+    kern<<<a.nv + (T::NTHR == 256 ? nfin : 0), T::NTHR, lds, s>>>(a);
     if (a.rsplit > 1) {
         const long nb = ((long)a.V * a.K + 1023) / 1024;
         const int g = (int)(nb > 2048 ? 2048 : nb);
@@ -1091,10 +1101,6 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
             default: rc = launch_dx<128, 32, 4, 1, 4>(d, s);
         }
         if (rc) return rc;
-        if (p.ns > 1 && p.wt < 2) {
-            const long nb = ((long)n * K + 1023) / 1024;
-            ce_dx_finish_kernel<<<(int)(nb > 2048 ? 2048 : nb), 256, 0, s>>>(d.slab, row, w, d.dx, n, K, p.ns);
-        }
 
         CeDwArgs c;
         c.xs = {xs, K, K}; c.e = {E, p.Vp, p.Vp};
