@@ -2439,12 +2439,12 @@ _HERE = _Here()
 
 def _on_device(t):
     """Launches go to the current device: make the tensors' device the current one (no cost where it already is)."""
-    return _HERE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    return _HERE if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
 
 
 def _stream_of(t):
     """The current stream of the tensors' device (the raw handle: torch.cuda.current_stream() builds an object first, 3 us)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _chk_out(t, n, dtypes, like, name):
@@ -2504,8 +2504,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
                 if t is not None:
                     t.zero_()
             return torch.zeros((), dtype=torch.float32, device=dev), dx, dw, db, torch.empty(0, dtype=torch.float32, device=dev)
-        out = torch.empty(N + 1, dtype=torch.float32, device=dev)
-        loss, rows = out[N], out[:N]
+        loss, rows = torch.empty((), dtype=torch.float32, device=dev), torch.empty(N, dtype=torch.float32, device=dev)
         bf = int(want_grad and dw.dtype == torch.bfloat16)
         nws = _dense_ce_ws(N, V, K, int(want_grad), bf, CE_PIECE_BYTES, CE_TILE)
         if nws < 0:
@@ -2519,6 +2518,8 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
 
 
 # ------------------------------------------------------------------------------ 8-bit activation checkpoints
+from .functional import Packed8  # noqa: E402  (functional imports this module when it is first called)
+
 _pack8 = _sig("ddl_pack8", ci, vp, vp, vp, cl, vp)
 _unpack8 = _sig("ddl_unpack8", ci, vp, vp, vp, cl, vp)
 _act_bwd8 = _sig("ddl_act_bwd8", ci, vp, vp, vp, vp, cl, ci, cf, vp)
@@ -2528,30 +2529,31 @@ WGRAD8_TILE = -1            # tile of dense_wgrad8: -1 = by the sizes (csrc/hip/
 
 
 def _chk_packed(q, name="q"):
-    n = q.codes.numel()
-    if not (q.codes.is_cuda and q.codes.dtype == torch.int8 and q.codes.is_contiguous() and q.scales.device == q.codes.device
-            and q.scales.dtype == torch.uint8 and q.scales.is_contiguous() and q.scales.numel() == ceil_div(n, 32)):
+    c, s = q.codes, q.scales
+    n = c.numel()
+    if not (c.is_cuda and c.dtype == torch.int8 and c.is_contiguous() and s.device == c.device and s.dtype == torch.uint8
+            and s.is_contiguous() and s.numel() == ceil_div(n, 32)):
         raise ValueError(f"{name}: codes must be contiguous int8 and scales uint8, one per 32 codes, on one device")
-    if q.codes.dim() < 1 or q.codes.shape[-1] % 8 or q.codes.data_ptr() % 8:
+    if c.dim() < 1 or c.shape[-1] % 8 or c.data_ptr() % 8:
         raise ValueError(f"{name}: channel dim must be a multiple of 8 and the codes 8-byte aligned")
     return n
 
 
 def pack8(x):
-    from .functional import Packed8
     _chk_act(x, "x")
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(ceil_div(x.numel(), 32), dtype=torch.uint8, device=x.device)
-    if x.numel():
+    n = x.numel()
+    codes = torch.empty_like(x, dtype=torch.int8)             # (torch.empty of a shape and a device: 1 us more)
+    scales = torch.empty(ceil_div(n, 32), dtype=torch.uint8, device=x.device)
+    if n:
         with _on_device(x):
-            _rc(_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), _stream_of(x)), "pack8")
+            _rc(_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, _stream_of(x)), "pack8")
             _done()
     return Packed8(codes, scales)
 
 
 def unpack8(q, out=None):
     n = _chk_packed(q)
-    y = torch.empty(q.codes.shape, dtype=torch.bfloat16, device=q.codes.device) if out is None else out
+    y = torch.empty_like(q.codes, dtype=torch.bfloat16) if out is None else out
     if out is not None:
         _chk_out(out, n, (torch.bfloat16,), q.codes, "out")
     if n:
