@@ -681,21 +681,22 @@ __global__ __launch_bounds__(256) void ce_dw_finish_kernel(const CeDwArgs a) {
     }
 }
 
-// dw for at most 64 NS rows, NS = 1 or 2 steps of the reduction: the kernel is its store (2 or 4 K V bytes) and what feeds
-// it.  A
-// wave keeps the E fragments of its 32 classes in registers and walks its share of the features (all of them, or fewer
-// when the classes alone do not make three blocks per CU) 64 at a time, x' through two LDS buffers (L2 serves it, every
-// block reads the same 64 x K).  64 x 2048 x 30000: 32 us, 3.9 TB/s of stores, where the tile product above took 47; 8 x
-// 1024 x 50000: 24 and 40.  The store counts as a memory
-// operation like the DMA: waiting for the next chunk leaves the STORES youngest operations, this chunk's stores, in
-// flight, which holds because every one of them is issued (out of range: past the descriptor, dropped).
-template <bool BF16, int NS>
-__global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const CeDwArgs a) {
+// dw for at most 64 rows, one step of the reduction: the kernel is its store (2 or 4 K V bytes) and what feeds it.  A wave
+// keeps the E fragments of its 32 classes in registers and walks its share of the features (all of them, or fewer when the
+// classes alone do not make three blocks per CU) 64 at a time, x' through two LDS buffers (L2 serves it, every block reads
+// the same 64 x K).  For up to 1024 features: a chunk of 128 bytes per class every few us spreads over more memory pages the
+// wider the rows are (8 x 1024 x 50000, bf16: 26 us, 3.9 TB/s, tiles 29; 64 x 512 x 3000 6.3 and 11; 32 x 1024 x 400000 176 and
+// 190; but 32 x 2048 x 65536 85 and 81, 8 x 4096 x 50000 121 and 92; chunks of 128 features 28, 9, 175, 98, 116).
+// The store counts as a memory operation like the DMA: waiting for the next chunk leaves the STORES youngest operations,
+// this chunk's stores, in flight, which holds because every one of them is issued (out of range: past the descriptor,
+// dropped).
+template <bool BF16>
+__global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
     constexpr int BV = 128, WV = 32, KC = 64, ES = BF16 ? 2 : 4, PITCH = KC * ES + 16;
     constexpr int STORES = WV * KC * ES / 16 / 64;
     using SE = GtStage<BV, 4, true>;
     using SX = GtStage<KC, 4, true>;
-    constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > NS * SE::BYTES ? PATCH : NS * SE::BYTES;
+    constexpr int PATCH = 4 * WV * PITCH, E_OR_PATCH = PATCH > SE::BYTES ? PATCH : SE::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];                       // [E, later the patches][x'][x']
     if ((int)blockIdx.x >= a.nv) {
         if (blockIdx.y == 0)
@@ -709,16 +710,14 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
     char* xbuf = smem + E_OR_PATCH;
     SE se;
     se.init(a.e, v0, 0, a.N, wave, lane);
-#pragma unroll
-    for (int n = 0; n < NS; ++n) se.issue(lds0 + n * SE::BYTES, wave);
+    se.issue(lds0, wave);
     int slots[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) slots[j] = wv + 16 * j + fr < a.V ? a.slot[wv + 16 * j + fr] : -1;
     auto fetch = [&](int k, int buf) {
         SX sx;
         sx.init(a.xs, k, 0, a.N, wave, lane);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) sx.issue(lds0 + E_OR_PATCH + (buf * NS + n) * SX::BYTES, wave);
+        sx.issue(lds0 + E_OR_PATCH + buf * SX::BYTES, wave);
         asm volatile("" ::: "memory");                       // the stores of this chunk stay behind the DMA of the next
     };
     const int nc = (a.K + KC - 1) / KC, share = (nc + gridDim.y - 1) / gridDim.y;
@@ -729,19 +728,19 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
     GtFrag<KC, true> fx;
     fe.init(wave * WV, lane);
     fx.init(0, lane);
-    bf16x8_t ev[2 * NS][2];
+    bf16x8_t ev[2][2];
 #pragma unroll
-    for (int kk = 0; kk < 2 * NS; ++kk)
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) ev[kk][j] = fe.load(smem + (kk >> 1) * SE::BYTES, j, kk & 1, wave * (WV / 16));
+        for (int j = 0; j < 2; ++j) ev[kk][j] = fe.load(smem, j, kk, wave * (WV / 16));
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");                 // E's LDS becomes the patches
 
     if (a.db && c0 == 0) {
         f32x4 b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < 2 * NS; ++kk) {
+        for (int kk = 0; kk < 2; ++kk) {
             const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            const s16x8 gv = kk * 32 < a.g2_pitch ? *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + kk * 32 + 8 * fq) : z;
+            const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + kk * 32 + 8 * fq);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
                 b = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, (fr & ~1) == 4 * j ? gv : z),
@@ -762,15 +761,15 @@ __global__ __launch_bounds__(256, NS == 1 ? 3 : 2) void ce_dw_thin_kernel(const 
     for (int c = c0; c < c1; ++c) {
         if (c > c0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(STORES) : "memory");
         fetch((c + 1) * KC, (c + 1) & 1);                     // past the share unused, past the last feature zeros
-        const char* xt = xbuf + (c & 1) * NS * SX::BYTES;
+        const char* xt = xbuf + (c & 1) * SX::BYTES;
         f32x4 acc[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < 2 * NS; ++kk)
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bf16x8_t xv = fx.load(xt + (kk >> 1) * SX::BYTES, i, kk & 1, 0);
+                const bf16x8_t xv = fx.load(xt, i, kk, 0);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, ev[kk][j], acc[i][j], 0, 0, 0);
@@ -901,8 +900,8 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
             }
         }
     }
-    // dw: the streaming kernel to 128 rows (100 x 1024 x 20000: 24 us, 128 x 4096 x 50000: 171, where the tiles took 28 and
-    // 203; with four steps, 200 x 1024 x 20000: 37 and 37, 256 x 2048 x 50000: 143 and 123)
+    // dw: the streaming kernel for one step and rows that are not too wide (both sides beside it; with two steps of rows, 100 x
+    // 1024 x 20000, 23 us and the tiles 21), else tiles
     // The tiles by their estimated time: a CU holds one 256 x 256 block or three of 128 x 128, which are out of step with one
     // another, so one's store runs under the others' products (stages of 32 rows: three blocks' LDS fits.  512 x 1024 x 50021:
     // 82 us, 256 x 256 tiles 96; 256 x 2048 x 50000: 110 and 132; 4096 x 2048 x 32768: 618 and 555; 8192 x 4096 x 131072: 10.8
@@ -912,10 +911,11 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         static const int edge[2] = {256, 128}, fit[2] = {1, 3};
         static const double round_us[2] = {1.75, 1.64}, one_us[2] = {1.75, 1.3}, ends[2] = {8.0, 3.5};
         const int steps = ce_cdiv(p.R, 64), forced = force_tile >= 0 ? force_tile / 100 % 10 : 9;
-        p.wt = p.R <= 64 ? 2 : 3; p.rs = 1; p.rper = steps * 64;
+        const bool thin = p.R <= 64 && K <= 1024;
+        p.wt = 2; p.rs = 1; p.rper = steps * 64;
         double best = 0;
         for (int t = 0; t < 2; ++t) {
-            if (forced < 2 ? t != forced : p.R <= 128) continue;
+            if (forced < 2 ? t != forced : thin) continue;
             const long tiles = (long)ce_cdiv(K, edge[t]) * ce_cdiv(V, edge[t]);
             for (int want = 1; want <= 32 && (want == 1 || want <= steps / 4); ++want) {
                 const int per = ce_cdiv(steps, want), n = ce_cdiv(steps, per);
@@ -1008,10 +1008,10 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     return gt_launched();
 }
 
-template <bool BF16, int NS>
+template <bool BF16>
 static int launch_dw_thin(CeDwArgs& a, hipStream_t s) {
-    const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = NS * 128 * 64 * 2, lds = (patch > e ? patch : e) + NS * 2 * 64 * 64 * 2;
-    constexpr auto kern = ce_dw_thin_kernel<BF16, NS>;
+    const size_t patch = 4 * 32 * (64 * (BF16 ? 2 : 4) + 16), e = 128 * 64 * 2, lds = (patch > e ? patch : e) + 2 * 64 * 64 * 2;
+    constexpr auto kern = ce_dw_thin_kernel<BF16>;
     if (int rc = gt_lds<kern>(lds)) return rc;
     const int nc = (a.K + 63) / 64;
     a.nv = (a.V + 127) / 128;
@@ -1119,8 +1119,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         switch (p.wt) {
             case 0: rc = launch_dw<256, 256, 2, 4, 2, 64>(c, s); break;
             case 1: rc = launch_dw<128, 128, 2, 2, 3, 32>(c, s); break;
-            case 2: rc = c.out_bf16 ? launch_dw_thin<true, 1>(c, s) : launch_dw_thin<false, 1>(c, s); break;
-            default: rc = c.out_bf16 ? launch_dw_thin<true, 2>(c, s) : launch_dw_thin<false, 2>(c, s);
+            default: rc = c.out_bf16 ? launch_dw_thin<true>(c, s) : launch_dw_thin<false>(c, s);
         }
         if (rc) return rc;
     }

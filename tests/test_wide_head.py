@@ -402,3 +402,36 @@ def test_padding_classes_are_zero_in_a_dirty_workspace(N, K, V):
         dirty = [torch.full((1 << s,), 255, dtype=torch.uint8, device="cuda") for s in (14, 16, 18, 20, 20, 21, 22)]
         del dirty                                              # NaN bits in the allocator's free blocks
         check(F.dense_softmax_ce(*d), exact(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", [(64, 1024, 300), (64, 1032, 300), (1, 1032, 70), (9, 2048, 515), (65, 1024, 200), (128, 1032, 333)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_rows_of_both_widths(N, K, V, dtype):
+    """Both sides of the rule that picks the weight gradient's kernel for few rows."""
+    a = make(N, K, V, seed=N + K, drop=0.1 if N > 4 else 0.0)
+    check(F.dense_softmax_ce(*cuda(*a), grad_dtype=dtype), exact(*a), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", [(5, 1024, 150001), (100, 1024, 150001), (200, 1024, 150001), (7, 4800, 30011)])
+def test_weights_larger_than_the_cache(N, K, V):
+    """More than 256 MiB of weights, read past the caches where one row tile is all there is.  Most classes are switched off, so
+    the definition needs only the others; what is switched off has gradients of exactly 0."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(N, K, generator=g, device="cuda").bfloat16()
+    w = torch.randn(V, K, generator=g, device="cuda", dtype=torch.bfloat16) * (1.5 / math.sqrt(K))
+    assert w.numel() * 2 > 256 << 20
+    on = torch.cat([torch.randperm(V, generator=g, device="cuda")[:500], torch.tensor([0, V - 1], device="cuda")]).unique()
+    b = torch.full((V,), -math.inf, device="cuda")
+    b[on] = torch.randn(on.numel(), generator=g, device="cuda") * 0.3
+    pick = torch.randint(0, on.numel(), (N,), generator=g, device="cuda")
+    loss, dx, dw, db, rows = F.dense_softmax_ce(x, w, b, on[pick])
+    ref = exact(x.cpu(), w[on].cpu(), b[on].cpu(), pick.cpu())
+    ref["V"] = V
+    check((loss, dx, dw[on], db[on], rows), ref)
+    off = torch.ones(V, dtype=torch.bool, device="cuda")
+    off[on] = False
+    assert int((dw[off] != 0).sum()) == 0 and int((db[off] != 0).sum()) == 0
+    score = F.dense_softmax_ce(x, w, b, on[pick], want_grad=False)
+    check((score[0], None, None, None, score[4]), ref)
