@@ -131,8 +131,20 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_l
     if (STORE && tb == 0)
         for (int i = tid; i < BA; i += T::NTHR)
             if (v0 + i < a.V) a.slot[v0 + i] = -1;
+    // the tile's biases (in powers of two; no class there: -inf, E = 0) and labels, one of each per thread: fetched here, their
+    // latency is the loop's, and handed round through LDS behind it (read where they are used: 512 x 1024 x 50021 71 us, 66 so,
+    // 2048 x 512 x 32000 99 and 87; all of a lane's own in registers across the loop: 74 and 101)
+    static_assert(BA <= T::NTHR && BB <= T::NTHR, "tile");
+    const float my_bias = tid < BA && v0 + tid < a.V && a.bias ? a.bias[v0 + tid] : 0.f;
+    const long my_label = tid < BB && r0 + tid < a.N ? a.labels[r0 + tid] : -1;
     f32x4 acc[T::NA][T::NB];
     T::run(a.w, a.x, v0, r0, 0, a.K, smem, acc, [](int, const bf16x8_t (&)[T::NB]) {});
+    constexpr int PITCH = BA * 2 + 16;
+    float* tile_bias = (float*)(smem + (STORE ? BB * PITCH : 0));      // behind E's patch, in the stages' place
+    int* tile_label = (int*)(tile_bias + BA);
+    if (tid < BA) tile_bias[tid] = v0 + tid < a.V ? my_bias * CE_LOG2E : -INFINITY;
+    if (tid < BB) tile_label[tid] = (unsigned long)my_label < (unsigned long)a.V ? (int)my_label : -1;
+    __syncthreads();
 
     const int lane = tid & 63, wave = tid >> 6, fr = lane & 15, fq = lane >> 4;
     const int wa = wave % WA, wb = wave / WA;
@@ -140,22 +152,16 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_l
     // The epilogue is as long as eight steps of the loop if every element pays for a maximum, a label test and a live test
     // (512 x 1024 x 50021: 75 us with them, 68 without), so the common case does a multiply-add, an exponential and a
     // sum per element; which wave tiles need more shows in the sum and in two votes.
-    float bias[T::NA][4];            // in powers of two; no class there: -inf, E = 0
+    f32x4 bias[T::NA];
 #pragma unroll
-    for (int i = 0; i < T::NA; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int v = wv + 16 * i + 4 * fq + e;
-            bias[i][e] = v < a.V ? (a.bias ? a.bias[v] * CE_LOG2E : 0.f) : -INFINITY;
-        }
-    constexpr int PITCH = BA * 2 + 16;
+    for (int i = 0; i < T::NA; ++i) bias[i] = *(const f32x4*)(tile_bias + wa * (BA / WA) + 16 * i + 4 * fq);
     char* lrow = smem + (size_t)(wb * (BB / WB)) * PITCH + wa * (BA / WA) * 2;
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int r = wr + 16 * j + fr;
-        const long lab = r < a.N ? a.labels[r] : -1;
-        const bool live = (unsigned long)lab < (unsigned long)a.V;
-        const int lrel = live ? (int)lab - wv - 4 * fq : -1;      // the label's position among this lane's classes
+        const int lab = tile_label[wb * (BB / WB) + 16 * j + fr];
+        const bool live = lab >= 0;
+        const int lrel = live ? lab - wv - 4 * fq : -1;           // the label's position among this lane's classes
         if (__any((unsigned)lrel < (unsigned)(BA / WA) && (lrel & 15) < 4)) {
             float zt = 0.f;
             bool mine = false;
@@ -945,8 +951,8 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
 template <int BA, int BB, int WA, int WB, int STAGES, bool STORE>
 static int launch_logits(CeLogitsArgs& a, hipStream_t s) {
     using T = GtTile<BA, BB, WA, WB, false, false, STAGES, GT_PLAIN>;
-    size_t lds = T::LDS_BYTES, out = (size_t)BB * (BA * 2 + 16);
-    if (STORE && out > lds) lds = out;
+    const size_t out = (STORE ? BB * (BA * 2 + 16) : 0) + (BA + BB) * 4;
+    size_t lds = out > T::LDS_BYTES ? out : T::LDS_BYTES;
     if (a.order && 4L * a.N > (long)lds) lds = 4L * a.N;
     constexpr auto kern = ce_logits_kernel<BA, BB, WA, WB, STAGES, STORE>;
     if (int rc = gt_lds<kern>(lds)) return rc;
