@@ -560,7 +560,7 @@ __device__ __forceinline__ float ce_label_bias(const CeDwArgs& a, int sl) {
 }
 
 template <int BA, int BB, int WA, int WB, int STAGES, int BK>
-__global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_dw_kernel(const CeDwArgs a) {
+__global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 3)) void ce_dw_kernel(const CeDwArgs a) {
     using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO, BK>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     if (T::NTHR == 256 && (int)blockIdx.x >= a.nv) {
@@ -576,15 +576,43 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     const bool do_db = ta == 0 && wa == 0;                     // wave-uniform
     f32x4 acc[T::NA][T::NB], bacc = {0.f, 0.f, 0.f, 0.f};
     static_assert(T::NB <= 4, "rows of the bias accumulator");
-    int slots[T::NB];                                          // fetched here: their latency is the loop's
+    int slots[T::NB];                                          // the classes' first label runs
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int v = v0 + wb * (BB / WB) + 16 * j + fr;
         slots[j] = v < a.V && !a.rslab ? a.slot[v] : -1;
     }
+    const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
+    // The sums start from the label terms, loaded while the first steps are on their way: behind the loop the loads of 16
+    // classes at a time waited for each other (2048 x 2048 x 32000: 304 us, 276 so; 512 x 1024 x 50021 82 and 77)
+    auto labels = [&](f32x4 (&c)[T::NA][T::NB]) {
+        int any = -1, next[T::NB];
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) any = max(any, slots[j]);
+        if (!__any(any >= 0)) return T::clear(c);
+        auto at = [&](int sl, int i) { return *(const f32x4*)(a.L + (long)sl * a.K + min(wk + 16 * i, a.K - 4)); };
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+            const int sl = max(slots[j], 0);                  // loaded whether there is one or not, and dropped
+            next[j] = a.next[sl];
+#pragma unroll
+            for (int i = 0; i < T::NA; ++i) c[i][j] = at(sl, i);
+        }
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j) {
+#pragma unroll
+            for (int i = 0; i < T::NA; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[i][j][e] = slots[j] >= 0 ? c[i][j][e] : 0.f;
+            for (int sl = slots[j] >= 0 ? next[j] : -1; __any(sl >= 0); sl = sl >= 0 ? a.next[sl] : -1)
+#pragma unroll
+                for (int i = 0; i < T::NA; ++i)
+                    if (sl >= 0) c[i][j] += at(sl, i);
+        }
+    };
     // db = E^T g: one more matrix instruction per B fragment j, against a fragment whose rows 4 j and 4 j + 1 are g's two
     // terms and all others zero: one accumulator holds all of them
-    T::run(a.xs, a.e, k0, v0, n0, n1, smem, acc, [&](int k, const bf16x8_t (&bv)[T::NB]) {
+    T::template run_from<false>(a.xs, a.e, k0, v0, n0, n1, smem, acc, labels, [&](int k, const bf16x8_t (&bv)[T::NB]) {
         if (do_db) {
             const s16x8 gv = *(const s16x8*)(a.g2 + (fr & 1) * a.g2_pitch + n0 + k + 8 * fq);
             const s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -595,7 +623,6 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
             }
         }
     });
-    const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
     // bf16 rows leave through the wave's own LDS patch as whole 16-byte groups (8-byte stores of 16 rows at a time: 17 -> 10
     // us of a batch of 32), past the caches: the next reader is the optimiser (the whole step of 1237 x 776 x 30011: 281 ->
     // 270 us, of 96 x 2048 x 60000 256 -> 224, of 512 x 1024 x 50021 228 -> 231)
@@ -619,10 +646,6 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     for (int j = 0; j < T::NB; ++j) {
         const int v = wv + 16 * j;
         if (v >= a.V) continue;
-        for (int sl = slots[j]; __any(sl >= 0); sl = sl >= 0 ? a.next[sl] : -1)       // most 16-class groups have no label
-#pragma unroll
-            for (int i = 0; i < T::NA; ++i)
-                if (sl >= 0 && wk + 16 * i < a.K) acc[i][j] += *(const f32x4*)(a.L + (long)sl * a.K + wk + 16 * i);
         if (do_db && fq == j && a.db) {
             float b = bacc[0] + bacc[1] + ce_label_bias(a, slots[j]);
             if (a.acc_b) b += a.acc_b[v];

@@ -178,13 +178,21 @@ struct GtTile {
     template <typename F>
     static __device__ __forceinline__ void run(const GtOperand& A, const GtOperand& B, int a0, int b0, int k0, int k1,
                                                char* smem, f32x4 (&acc)[NA][NB], F&& per_half) {
-        if (BB <= 128 && A.once) run_as<true>(A, B, a0, b0, k0, k1, smem, acc, per_half);
-        else run_as<false>(A, B, a0, b0, k0, k1, smem, acc, per_half);
+        auto zero = [](f32x4 (&c)[NA][NB]) { clear(c); };
+        if (BB <= 128 && A.once) run_from<true>(A, B, a0, b0, k0, k1, smem, acc, zero, per_half);
+        else run_from<false>(A, B, a0, b0, k0, k1, smem, acc, zero, per_half);
     }
+    static __device__ __forceinline__ void clear(f32x4 (&c)[NA][NB]) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) c[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    // init(acc): what the sums start from, called while the first steps are on their way
     // two loops: a branch at every issue cost the tiles of 128 rows 2 %
-    template <bool ONCE, typename F>
-    static __device__ __forceinline__ void run_as(const GtOperand& A, const GtOperand& B, int a0, int b0, int k0, int k1,
-                                               char* smem, f32x4 (&acc)[NA][NB], F&& per_half) {
+    template <bool ONCE, typename I, typename F>
+    static __device__ __forceinline__ void run_from(const GtOperand& A, const GtOperand& B, int a0, int b0, int k0, int k1,
+                                               char* smem, f32x4 (&acc)[NA][NB], I&& init, F&& per_half) {
         const int lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wa = wave % WA, wb = wave / WA;
@@ -195,17 +203,13 @@ struct GtTile {
         fa.init(wa * (BA / WA), lane);
         fb.init(wb * (BB / WB), lane);
         const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) char*)smem;
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
         const int nsteps = (k1 - k0 + BK - 1) / BK;
 #pragma unroll
         for (int d = 0; d < STAGES - 1; ++d) {
             sa.template issue<ONCE>(lds0 + d * STAGE_BYTES, wave);
             sb.issue(lds0 + d * STAGE_BYTES + SA::BYTES, wave);
         }
+        init(acc);
         int cur = 0, nxt = STAGES - 1;
         for (int s = 0; s < nsteps; ++s) {
             // this wave's share of step s has landed and its reads of the buffer that is refilled below have returned;
