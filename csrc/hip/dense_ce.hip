@@ -904,8 +904,18 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         if (r > CE_MAX_ROWS) r = CE_MAX_ROWS;
         if (p.R > r) p.R = (int)r;
     }
-    // as few padding rows as the batch leaves, and enough blocks for 256 CUs
-    p.lt = p.R <= 32 ? (V < 256 * 128 ? 3 : 2) : (p.R <= 128 || (long)ce_cdiv(V, 256) * ce_cdiv(p.R, 256) < 256 ? 1 : 0);
+    // logits: up to 32 rows the tiles that pad them least, the small ones for enough blocks; else by the estimated time, 64-deep
+    // steps plus a block's ends in rounds of one 256 x 256 block or two of 128 x 128 per CU (700 x 2400 x 20000 67 and 91 us,
+    // 256 x 2048 x 50000 57 and 75, 256 x 1024 x 30000 33 and 26, 300 x 512 x 20000 23 and 17)
+    if (p.R <= 32) {
+        p.lt = V < 256 * 128 ? 3 : 2;
+    } else {
+        const int steps = ce_cdiv(K, 64);
+        const double two = ce_cdiv((long)ce_cdiv(V, 128) * ce_cdiv(p.R, 128), 256) * 0.5;
+        const double us0 = ce_cdiv((long)ce_cdiv(V, 256) * ce_cdiv(p.R, 256), 256) * (steps * 1.6 + 6.0);
+        const double us1 = (two > 0.75 ? two : 0.75) * (steps * 1.1 + 5.0);
+        p.lt = us0 < us1 ? 0 : 1;
+    }
     if (force_tile >= 0 && force_tile % 10 < 4) p.lt = force_tile % 10;
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
     p.wave_cols = cols[p.lt];
