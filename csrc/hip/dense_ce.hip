@@ -920,12 +920,13 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
     p.wave_cols = cols[p.lt];
     p.nst = ce_cdiv(p.Vp, ba[p.lt]) * (ba[p.lt] / p.wave_cols);      // the tiles cover E's zero columns too
-    // dx: the tile and the number of splits over the classes by their estimated time: whole rounds of the chip (one 256 x
-    // 256 block or two 128 x 128 / four 128 x 32 blocks per CU) of 64-deep steps plus a block's start and end, and the
-    // splits' fp32 partial sums written and read once
+    // dx: the tile and the number of splits over the classes by their estimated time: blocks per CU (one of 256 x 256 at
+    // a time or two of the others, which are slower each and faster alone) of 64-deep steps plus a block's start and end, and
+    // the splits' fp32 partial sums written and read once (in whole rounds of two: 1000 x 512 x 10000 83 us, 76 so; 32 x 2048
+    // x 65536 190 and 182)
     {
-        static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32}, slots[3] = {256, 512, 1024};
-        static const double step_us[3] = {1.75, 1.05, 0.7}, ends = 4.0;
+        static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32};
+        static const double block_us[3] = {1.75, 0.525, 0.35}, least_us[3] = {1.75, 0.79, 0.5}, ends = 4.0;
         const int steps = ce_cdiv(V, 64), forced = force_tile >= 0 ? force_tile / 10 % 10 : 9;
         double best = 0;
         for (int t = 0; t < 3; ++t) {
@@ -933,8 +934,8 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
             const long tiles = (long)ce_cdiv(K, xa[t]) * ce_cdiv(p.R, xb[t]);
             for (int ns = 1; ns <= 64 && (ns == 1 || ns <= steps / 4); ++ns) {
                 const int per = ce_cdiv(steps, ns), n = ce_cdiv(steps, per);
-                const double rounds = (double)ce_cdiv(tiles * n, slots[t]);
-                const double us = rounds * (per + ends) * step_us[t] + (n > 1 ? 4.0 + n * 8.0 * p.R * K / 4.5e6 : 0.0);
+                const double share = ce_cdiv(tiles * n, 256) * block_us[t];
+                const double us = (share > least_us[t] ? share : least_us[t]) * (per + ends) + (n > 1 ? 4.0 + n * 8.0 * p.R * K / 4.5e6 : 0.0);
                 if (best == 0 || us < best) { best = us; p.xt = t; p.ns = n; p.per = per * 64; }
             }
         }
