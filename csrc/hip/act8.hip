@@ -394,14 +394,15 @@ static int launch_wgrad8(Wg8Args& a, hipStream_t s) {
     return gt_launched();
 }
 
-// Tile and row splits of a call, by their estimated time: whole rounds of the chip (blocks that fit it) of 64-row steps plus a
-// block's start and end, the splits' partial sums written and read once, and the unpacking.  Reading the codes in the product
-// saves 3 bytes per element of x but costs 2.5 vector instructions per element and output tile: 1000 x 6272 x 128 20 us
-// (unpacked first: 28), 512 x 1024 x 1024 17 (22), 4096 x 2048 x 2048 65 (62), 16384 x 4096 x 4096 586 (496).
+// Tile and row splits of a call, by their estimated time: 64-row steps plus a block's start and end in rounds of the blocks
+// that share a CU (1000 x 6272 x 128, 196 tiles: one block per CU 15.5 us, 4 splits and as many blocks per CU 18.7), the
+// splits' partial sums written and read once, and the unpacking.  Reading the codes in the product saves 3 bytes per element
+// of x but costs 2.5 vector instructions per element and output tile (kernels' time: 1000 x 6272 x 128 20 us, unpacked first
+// 27; 512 x 1024 x 1024 12 and 16; 4096 x 2048 x 2048 77 and 62; 16384 x 4096 x 4096 854 and 487).
 struct Wg8Plan { int tile, ns, per; };                       // tile: see ddl_dense_wgrad8
 static Wg8Plan wg8_plan(int R, int K, int O, int force) {
-    static const int edge[4] = {64, 128, 128, 256}, slots[4] = {1024, 512, 512, 256};
-    static const double step_us[4] = {1.35, 1.78, 1.25, 1.75};
+    static const int edge[4] = {64, 128, 128, 256}, fit[4] = {4, 2, 2, 1};      // blocks that share a CU,
+    static const double step_us[4][4] = {{0.67, 0.8, 1.06, 1.28}, {1.42, 1.78}, {1.1, 1.2}, {1.75}};      // and a step of so many
     const int steps = (R + 63) / 64;
     Wg8Plan p = {0, 1, steps * 64};
     double best = 0;
@@ -410,8 +411,9 @@ static Wg8Plan wg8_plan(int R, int K, int O, int force) {
         const long tiles = (long)((K + edge[t] - 1) / edge[t]) * ((O + edge[t] - 1) / edge[t]);
         for (int want = 1; want <= 64 && (want == 1 || want <= steps / 4); ++want) {
             const int per = (steps + want - 1) / want, ns = (steps + per - 1) / per;
-            const double us = (double)((tiles * ns + slots[t] - 1) / slots[t]) * (per + 4.0) * step_us[t] +
-                              (ns > 1 ? 3.0 + 0.15 * ns + ns * 8.0 * O * K / 4.5e6 : 0.0) +
+            const long cu = (tiles * ns + 255) / 256, rest = cu % fit[t];
+            const double us = (cu / fit[t] * step_us[t][fit[t] - 1] + (rest ? step_us[t][rest - 1] : 0.0)) * (per + 4.0) +
+                              (ns > 1 ? 2.5 + ns * 8.0 * O * K / 7e6 : 0.0) +
                               (t >= 2 ? 4.0 + 3.0 * R * K / 4.5e6 : 0.0);
             if (best == 0 || us < best) { best = us; p = {t, ns, per * 64}; }
         }
