@@ -334,10 +334,16 @@ __global__ __launch_bounds__(NTHR) void ce_rows_kernel(const CeRowsArgs a) {
 
 // mean of the row losses over the labelled rows, fp64 in a fixed order; one block of NTHR threads
 template <int NTHR>
-__device__ __forceinline__ void ce_mean(const float* rows, const float* count, int N, float* loss) {
-    __shared__ double red[NTHR / 64];
+__device__ __forceinline__ void ce_mean(const float* rows, const float* count, int N, float* loss, double (&red)[NTHR / 64]) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < N; i += NTHR) s += (double)rows[i];
+    constexpr int U = 8;                                      // loads in flight (one at a time: 56 us of 8000 x 64 x 65)
+    for (int i = threadIdx.x; i < N; i += NTHR * U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = rows[min(i + u * NTHR, N - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u) s += i + u * NTHR < N ? (double)v[u] : 0.0;
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -349,7 +355,8 @@ __device__ __forceinline__ void ce_mean(const float* rows, const float* count, i
     }
 }
 __global__ __launch_bounds__(1024) void ce_mean_kernel(const float* rows, const float* count, int N, float* loss) {
-    ce_mean<1024>(rows, count, N, loss);
+    __shared__ double red[16];
+    ce_mean<1024>(rows, count, N, loss, red);
 }
 
 // Scoring a few rows of few tiles: row losses (a wave each) and their mean in one block instead of two launches.  With
@@ -374,14 +381,15 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
         if (lane == 0) a.rows[r] = v;
     }
     __syncthreads();
-    ce_mean<1024>(a.rows, a.count, a.N, loss);
+    __shared__ double red[16];
+    ce_mean<1024>(a.rows, a.count, a.N, loss, red);
 }
 
 // ------------------------------------------------------------------------------------------------ 3. label terms
 // Rows in sorted order, in windows of 64 positions: the rows of one class inside a window are a run; its first position i
 // sums it (ascending) into L[i], and next[i] is the window where the class goes on, or -1.  slot[class] is its first run.
 // Windows bound a block's work whatever the labels are (8000 rows, 1000 of them of one class: 340 us with a block per class,
-// 20 so).  Eight features per thread, 256 threads.  Position n, behind them all, takes the mean of the row losses.
+// 20 so).  256 threads.  Block 0, in front of them all, takes the mean of the row losses.
 #define CE_RUN 64
 struct CeLabelsArgs {
     const CeRow* row; const int* order; const bf16_t* x; const bf16_t* xs; int N, K;
@@ -389,16 +397,23 @@ struct CeLabelsArgs {
     const float* rows_all; const float* count; int n_all; float* loss;      // loss nullptr: not the last piece
 };
 
-__device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chunk) {
-    if (i == a.N) {
-        if (a.loss && chunk == 0) ce_mean<256>(a.rows_all, a.count, a.n_all, a.loss);
+// LDS of a block (the caller's: static LDS here would be every dx tile's, and cost the small ones their second block per CU)
+struct CeLabelsLds { union { double mean[4]; struct { float s[256][8]; float b[256]; }; }; };
+
+__device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chunk, CeLabelsLds& lds) {
+    if (i == 0) {                                             // (the longest block starts first)
+        if (a.loss && chunk == 0) ce_mean<256>(a.rows_all, a.count, a.n_all, a.loss, lds.mean);
         return;
     }
+    --i;
     const int lab = a.row[a.order[i]].label;
     if (lab < 0) return;
     const bool fresh = i == 0 || a.row[a.order[i - 1]].label != lab;
     if (!fresh && i % CE_RUN != 0) return;
-    const int k = (chunk * 256 + threadIdx.x) * 8, lane = threadIdx.x & 63;
+    int width = 8;
+    while (width < 256 && width * 8 < a.K) width *= 2;
+    const int tid = threadIdx.x, lane = tid & 63, g = tid / width;
+    const int k = (chunk * 256 + (tid & (width - 1))) * 8;
     const bool on = k < a.K;
     const int end = min((i / CE_RUN + 1) * CE_RUN, a.N);      // of the window
     const int q = i + lane < end ? a.order[i + lane] : a.order[i];
@@ -406,20 +421,24 @@ __device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chun
     const unsigned long m = __ballot(i + lane < end && c.label == lab);
     const int n = m == ~0ul ? 64 : __builtin_ctzl(~m);        // the run's rows are the leading lanes
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, b = 0.f;
-    constexpr int U = 8;
-    for (int j0 = 0; j0 < n; j0 += U) {                       // U rows' loads in flight, added in row order
+    // eight features per thread; threads that they leave over share the run's rows: group g of G takes rows g, g + G, ..
+    // (a row is 0.6 us of one wave: the whole step of 8000 x 64 x 65 took 123 us with G = 1, 88 so)
+    constexpr int U = 4;
+    const int G = min(256 / width, (n + U - 1) / U);
+    for (int j0 = 0; j0 < n; j0 += U * G) {
         uint4 xv[U], xr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long r = __builtin_amdgcn_readlane(q, min(j0 + u, n - 1));
-            xv[u] = on ? *(const uint4*)(a.x + r * a.K + k) : make_uint4(0, 0, 0, 0);
-            xr[u] = on ? *(const uint4*)(a.xs + r * a.K + k) : make_uint4(0, 0, 0, 0);
+            const long r = __shfl(q, min(j0 + u * G + g, n - 1), 64);
+            xv[u] = *(const uint4*)(a.x + r * a.K + (on ? k : 0));
+            xr[u] = *(const uint4*)(a.xs + r * a.K + (on ? k : 0));
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (j0 + u >= n) break;
-            const float tg = __shfl(c.tg, j0 + u, 64), hi = __shfl(c.hi, j0 + u, 64);
-            b += __shfl(c.rest, j0 + u, 64);
+            const int j = j0 + u * G + g, l = min(j, n - 1);
+            const float t = __shfl(c.tg, l, 64), h = __shfl(c.hi, l, 64), rest = __shfl(c.rest, l, 64);
+            const float tg = j < n ? t : 0.f, hi = j < n ? h : 0.f;
+            b += j < n ? rest : 0.f;
             float fv[8], fr[8];
             unpack8(xv[u], fv);
             unpack8(xr[u], fr);
@@ -427,18 +446,33 @@ __device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chun
             for (int e = 0; e < 8; ++e) s[e] += fmaf(tg, fv[e], -(hi * fr[e]));
         }
     }
-    if (on) {
+    if (G > 1) {                                              // the groups' sums, in order
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lds.s[tid][e] = s[e];
+        lds.b[tid] = b;
+        __syncthreads();
+        if (g > 0) return;
+        for (int o = tid + width; o < G * width; o += width) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += lds.s[o][e];
+            b += lds.b[o];
+        }
+    }
+    if (on && g == 0) {
         float* o = a.L + (long)i * a.K + k;
         *(float4*)o = make_float4(s[0], s[1], s[2], s[3]);
         *(float4*)(o + 4) = make_float4(s[4], s[5], s[6], s[7]);
     }
-    if (chunk == 0 && threadIdx.x == 0) {
+    if (chunk == 0 && tid == 0) {
         if (fresh) a.slot[lab] = i;
         a.Lb[i] = b;
         a.next[i] = end < a.N && a.row[a.order[end]].label == lab ? end : -1;
     }
 }
-__global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) { ce_labels(a, blockIdx.x, blockIdx.y); }
+__global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) {
+    __shared__ CeLabelsLds lds;
+    ce_labels(a, blockIdx.x, blockIdx.y, lds);
+}
 
 // ------------------------------------------------------------------------------------------------ 4. dx
 struct CeDxArgs {
@@ -470,7 +504,7 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_d
     extern __shared__ __attribute__((aligned(16))) char smem[];
     if (T::NTHR == 256 && (int)blockIdx.x >= a.ntile) {
         const int b = blockIdx.x - a.ntile, i = b / a.nlab_chunks;
-        ce_labels(a.lab, i, b - i * a.nlab_chunks);
+        ce_labels(a.lab, i, b - i * a.nlab_chunks, *(CeLabelsLds*)smem);
         return;
     }
     int ta, tb, split;
@@ -926,7 +960,7 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     // x 65536 190 and 182)
     {
         static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32};
-        static const double block_us[3] = {1.75, 0.525, 0.35}, least_us[3] = {1.75, 0.79, 0.5}, ends = 4.0;
+        static const double block_us[3] = {1.75, 0.525, 0.3}, least_us[3] = {1.75, 0.79, 0.35}, ends = 4.0;
         const int steps = ce_cdiv(V, 64), forced = force_tile >= 0 ? force_tile / 10 % 10 : 9;
         double best = 0;
         for (int t = 0; t < 3; ++t) {
