@@ -5,7 +5,7 @@
 //   dl = (softmax(z) - onehot) / count                  dx = dl w      dw = dl^T x      db = sum_r dl
 //
 // Three matrix products, 6 N K V operations, no recomputation.  Rows are taken in pieces whose workspace (2 bytes per
-// row and class) is bounded by the caller; scoring keeps nothing at all.
+// row and class; scoring: 8 per row and wave tile) is bounded by the caller.
 //
 //  1. `ce_logits`: z tile = w x^T on the matrix cores; the epilogue turns it into E = 2^{z log2(e) - c} and per row and
 //     wave tile the sum of the fp32 E.  E is stored in bf16 (the precision a bf16 gradient of the logits would have).
@@ -954,6 +954,11 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
     p.wave_cols = cols[p.lt];
     p.nst = ce_cdiv(p.Vp, ba[p.lt]) * (ba[p.lt] / p.wave_cols);      // the tiles cover E's zero columns too
+    if (!train && 8L * p.R * p.nst > budget) {                       // scoring keeps 8 bytes per row and wave tile
+        const long r = budget / (8L * p.nst) / 256 * 256;
+        p.R = (int)(r > 256 ? r : 256);
+        if (p.R > N) p.R = N;
+    }
     // dx: the tile and the number of splits over the classes by their estimated time: blocks per CU (one of 256 x 256 at
     // a time or two of the others, which are slower each and faster alone) of 64-deep steps plus a block's start and end, and
     // the splits' fp32 partial sums written and read once (in whole rounds of two: 1000 x 512 x 10000 83 us, 76 so; 32 x 2048
@@ -1145,15 +1150,16 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch; b.loss = nullptr;
         const bool wide = n <= 256 && p.nst > 512;            // few long rows: 1024 threads each (16 -> 6 us at 4096 entries)
         if (!train) {
-            if (n <= CE_FEW_ROWS && p.nst <= CE_FEW_STATS) {
+            if (N <= CE_FEW_ROWS && p.nst <= CE_FEW_STATS) {
                 ce_score_few_kernel<<<1, 1024, 0, s>>>(b, loss);
                 return gt_launched();
             }
-            if (n == 1) b.loss = loss;
+            if (N == 1) b.loss = loss;
             if (wide) ce_rows_kernel<false, 1024><<<n, 1024, 0, s>>>(b);
             else ce_rows_kernel<false, 256><<<n, 256, 0, s>>>(b);
-            if (n > 1) ce_mean_kernel<<<1, 1024, 0, s>>>(rows, count, N, loss);
-            return gt_launched();
+            if (last && N > 1) ce_mean_kernel<<<1, 1024, 0, s>>>(rows, count, N, loss);
+            if (int e = gt_launched()) return e;
+            continue;
         }
         if (wide) ce_rows_kernel<true, 1024><<<n, 1024, 0, s>>>(b);
         else ce_rows_kernel<true, 256><<<n, 256, 0, s>>>(b);

@@ -435,3 +435,27 @@ def test_weights_larger_than_the_cache(N, K, V):
     assert int((dw[off] != 0).sum()) == 0 and int((db[off] != 0).sum()) == 0
     score = F.dense_softmax_ce(x, w, b, on[pick], want_grad=False)
     check((score[0], None, None, None, score[4]), ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [257, 600, 1024])
+def test_scored_row_pieces(N, monkeypatch):
+    """A workspace that holds the statistics of 256 rows at a time: the same row losses, and the mean over all of them."""
+    from distributeddeeplearning_amd.ops import hip
+    a = make(N, 72, 700, seed=N, drop=0.1)
+    d = cuda(*a)
+    whole = F.dense_softmax_ce(*d, want_grad=False)
+    monkeypatch.setattr(hip, "CE_PIECE_BYTES", 1024)
+    out = F.dense_softmax_ce(*d, want_grad=False)
+    check(out, exact(*a))
+    assert torch.equal(out[4], whole[4]) and torch.equal(out[0], whole[0])
+
+
+@pytest.mark.gpu
+def test_gradient_over_the_weights_is_refused():
+    x, w, b, lab = cuda(*make(8, 16, 80))
+    both = torch.zeros(88, 16, dtype=torch.bfloat16, device="cuda")
+    both[:80] = w
+    for args in (dict(w=w, out_dw=w), dict(w=both[:80], out_dw=both[8:]), dict(x=both[80:], w=w, out_dw=both[8:])):
+        with pytest.raises(ValueError):
+            F.dense_softmax_ce(**{**dict(x=x, bias=b, labels=lab), **args})
