@@ -245,10 +245,11 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
     """Dense(K -> V) + softmax cross entropy for any number of classes, forward and backward, without the logits.
 
     x [N][K], w [V][K] (device: bf16, K padded to a multiple of 8 with zero lanes), bias [V] fp32 or None (-inf switches
-    a class off), labels [N] int64.  A row whose label is negative takes no part, whatever its x holds: row loss 0, dx 0,
-    not counted.  Returns (loss, dx, dw, db, rows): the mean over the labelled rows (0 if there are none), the gradients
-    of that mean (None without `want_grad`; db None without a bias) and the row losses.  dx has x's type, dw [V][K] and
-    db [V] `grad_dtype` (fp32 | bf16), or they overwrite `out_dw` / `out_db` in those tensors' type.
+    a class off; on the device so does anything below -2.3e38, the type's lowest value among it), labels [N] int64.  A row
+    whose label is negative takes no part, whatever its x holds: row loss 0, dx 0, not counted.  Returns (loss, dx, dw, db,
+    rows): the mean over the labelled rows (0 if there are none), the gradients of that mean (None without `want_grad`; db
+    None without a bias) and the row losses.  dx has x's type, dw [V][K] and db [V] `grad_dtype` (fp32 | bf16), or they
+    overwrite `out_dw` / `out_db` in those tensors' type (out_dw apart from w and x).
 
     A label past the last class makes its row loss (and the mean) NaN and its row no gradient; a labelled row with a NaN
     or infinite logit, or with every class switched off, has NaN loss and gradients.  On the device the gradient of the
@@ -301,9 +302,8 @@ class Packed8:
 
 def pack8(x):
     """Activation tensor -> Packed8 (33 bytes per 32 elements).  Per 32 elements the scale is the smallest power of two
-    from 2^-119 to
-    2^121 with max |x| <= 127 scale; codes round to nearest even, except that no non-zero value becomes 0 and the largest
-    bf16 number stays finite."""
+    from 2^-119 to 2^121 with max |x| <= 127 scale; codes round to nearest even, except that no non-zero value becomes 0
+    and the largest bf16 number stays finite."""
     return _b(x).pack8(x)
 
 

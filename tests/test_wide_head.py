@@ -459,3 +459,13 @@ def test_gradient_over_the_weights_is_refused():
     for args in (dict(w=w, out_dw=w), dict(w=both[:80], out_dw=both[8:]), dict(x=both[80:], w=w, out_dw=both[8:])):
         with pytest.raises(ValueError):
             F.dense_softmax_ce(**{**dict(x=x, bias=b, labels=lab), **args})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V", [(9, 300), (200, 1500)])
+def test_lowest_value_switches_a_class_off(N, V):
+    """A mask of the type's lowest value: the same bits as one of -inf (the labels' own classes stay on)."""
+    x, w, b, lab = make(N, 40, V, seed=N, mask=0.5)
+    low = torch.where(torch.isfinite(b), b, torch.full_like(b, torch.finfo(torch.float32).min))
+    for p, q in zip(F.dense_softmax_ce(*cuda(x, w, b, lab)), F.dense_softmax_ce(*cuda(x, w, low, lab))):
+        assert torch.equal(p, q)
