@@ -156,7 +156,7 @@ struct GtFrag {
 
 // The block's tile: BA x BB outputs, WA x WB waves.  Lane (fr, fq) of fragment pair (i, j) holds
 // D[wave_a0 + 16 i + 4 fq + e][wave_b0 + 16 j + fr], e = 0..3.
-// SCHED: what keeps the fragment reads and the matrix instructions of a half step apart.  One box, 8192 x 4096 x 32768,
+// SCHED: what keeps the fragment reads and the matrix instructions of a half step apart.  One run, 8192 x 4096 x 32768,
 // TFLOP/s of the three products (row x row, column x row, column x column order), each DMA split as below:
 //   0 nothing            1258  1278  1080
 //   1 raised priority    1210  1236  1221
