@@ -939,8 +939,10 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         if (p.R > r) p.R = (int)r;
     }
     // logits: up to 32 rows the tiles that pad them least, the small ones for enough blocks; else by the estimated time, 64-deep
-    // steps plus a block's ends in rounds of one 256 x 256 block or two of 128 x 128 per CU (700 x 2400 x 20000 67 and 91 us,
-    // 256 x 2048 x 50000 57 and 75, 256 x 1024 x 30000 33 and 26, 300 x 512 x 20000 23 and 17)
+    // steps plus a block's ends in rounds of one 256 x 256 block or two of 128 x 128 or 128 x 32 per CU (the large and the
+    // middle ones: 700 x 2400 x 20000 67 and 91 us, 256 x 2048 x 50000 57 and 75, 256 x 1024 x 30000 33 and 26, 300 x 512 x
+    // 20000 23 and 17; the middle and the small ones: 64 x 1024 x 10007 18 and 9, 64 x 2048 x 30000 34 and 22, 96 x 2048 x
+    // 60000 48 and 58)
     if (p.R <= 32) {
         p.lt = V < 256 * 128 ? 3 : 2;
     } else {
@@ -948,7 +950,9 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         const double two = ce_cdiv((long)ce_cdiv(V, 128) * ce_cdiv(p.R, 128), 256) * 0.5;
         const double us0 = ce_cdiv((long)ce_cdiv(V, 256) * ce_cdiv(p.R, 256), 256) * (steps * 1.6 + 6.0);
         const double us1 = (two > 0.75 ? two : 0.75) * (steps * 1.1 + 5.0);
-        p.lt = us0 < us1 ? 0 : 1;
+        const int small = ce_cdiv((long)ce_cdiv(V, 128) * ce_cdiv(p.R, 32), 256);
+        const double us2 = small > 1 ? small * 0.5 * (steps * 0.6 + 2.5) : steps * 0.27 + 2.5;
+        p.lt = us2 < us0 && us2 < us1 ? 2 : us0 < us1 ? 0 : 1;
     }
     if (force_tile >= 0 && force_tile % 10 < 4) p.lt = force_tile % 10;
     static const int ba[4] = {256, 128, 128, 32}, cols[4] = {128, 64, 32, 16};
@@ -962,14 +966,14 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     // dx: the tile and the number of splits over the classes by their estimated time: blocks per CU (one of 256 x 256 at
     // a time or two of the others, which are slower each and faster alone) of 64-deep steps plus a block's start and end, and
     // the splits' fp32 partial sums written and read once (in whole rounds of two: 1000 x 512 x 10000 83 us, 76 so; 32 x 2048
-    // x 65536 190 and 182)
+    // x 65536 190 and 182).  128 x 128 and 128 x 32: 64 x 2048 x 30000 25 and 21 us, 64 x 4096 x 50000 66 - 80 and 100 - 106
     {
         static const int xa[3] = {256, 128, 128}, xb[3] = {256, 128, 32};
-        static const double block_us[3] = {1.75, 0.525, 0.3}, least_us[3] = {1.75, 0.79, 0.35}, ends = 4.0;
+        const double block_us[3] = {1.75, 0.525, p.R <= 32 ? 0.3 : 0.34}, least_us[3] = {1.75, 0.79, 0.35}, ends = 4.0;
         const int steps = ce_cdiv(V, 64), forced = force_tile >= 0 ? force_tile / 10 % 10 : 9;
         double best = 0;
         for (int t = 0; t < 3; ++t) {
-            if (forced < 3 ? t != forced : (t == 2) != (p.R <= 32)) continue;
+            if (forced < 3 ? t != forced : t < 2 && p.R <= 32) continue;
             const long tiles = (long)ce_cdiv(K, xa[t]) * ce_cdiv(p.R, xb[t]);
             for (int ns = 1; ns <= 64 && (ns == 1 || ns <= steps / 4); ++ns) {
                 const int per = ce_cdiv(steps, ns), n = ce_cdiv(steps, per);
