@@ -32,6 +32,7 @@
 
 #define CE_LOG2E 1.44269504088896340736f
 #define CE_LN2 0.69314718055994530942f
+#define CE_LN2_REST -2.12194440054690583e-4f      // log 2 - 355 / 512
 constexpr long CE_CACHE = 256L << 20;      // the last level cache, shared by the whole chip
 constexpr int CE_NT = 2;                   // a raw buffer store's policy: non-temporal
 
@@ -231,6 +232,7 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_l
 struct CeRowsArgs {
     const float2* stats; int nst; int wave_cols;      // classes per stats entry
     const float* zt; const long* labels; const float* count;
+    const bf16_t* w; const float* bias;
     int N, V, K, Vp;
     bf16_t* E; const bf16_t* x; bf16_t* xs;           // xs = bf16(g x)
     float* rows; CeRow* row; bf16_t* g2; int g2_pitch;      // g2[0] + g2[1] = g in two bf16 terms, zero behind row N
@@ -240,10 +242,41 @@ struct CeRowsArgs {
 // 2^d for whole d, exact (0 below the normal range: such a term is 2^-126 of the row's largest)
 __device__ __forceinline__ float ce_pow2(float d) { return d < -126.f ? 0.f : ldexpf(1.f, (int)d); }
 
-// loss of a row from its reference, its sum and its label's logit
+// Loss of a row from its reference, its sum and its label's logit: log(S 2^cref) - zt.  With S = m 2^e the whole powers of two
+// leave as (e + cref) log 2 in two terms (355 / 512 and the rest, Cody and Waite: the first product is exact below 2^15), so
+// the difference is rounded at its own size, not at that of the logarithm (rows of 9 x 1958 x 156: 1.1e-6 -> 7e-7 off).
 __device__ __forceinline__ float ce_row_loss(float cref, float S, float zt) {
-    const float lse = __logf(S) + cref * CE_LN2;
-    return lse < INFINITY ? lse - zt : NAN;
+    if (!(S >= 0x1p-126f && S < INFINITY)) {                  // no class left, or a logit that is not finite
+        const float lse = __logf(S) + cref * CE_LN2;
+        return lse < INFINITY ? lse - zt : NAN;
+    }
+    const unsigned b = __float_as_uint(S) - 0x3f350000u;      // m in [0.707, 1.414)
+    const float m = __uint_as_float((b & 0x7fffffu) + 0x3f350000u), n = (float)((int)b >> 23) + cref;
+    return fmaf(n, 355.f / 512.f, -zt) + (__logf(m) + n * CE_LN2_REST);
+}
+
+// The label's logit once more, by a tree: the products' chain of K / 32 additions is most of a row loss' error (9 x 1958 x 156:
+// 7e-7, so 2e-7, plain fp32 3e-7; 300 x 4096 x 3000: 5e-7, 0.9e-7, 1e-6; 1 us of a step).  This thread's part of x_r w_label
+__device__ __forceinline__ float ce_label_dot(const CeRowsArgs& a, int r, long lab, int t, int threads) {
+    float d = 0.f;
+    for (int k = t * 8; k < a.K; k += threads * 8) {
+        float f[8], g[8];
+        unpack8(*(const uint4*)(a.x + (long)r * a.K + k), f);
+        unpack8(*(const uint4*)(a.w + lab * a.K + k), g);
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = fmaf(f[e], g[e], f[e + 4] * g[e + 4]);
+        d += (p[0] + p[1]) + (p[2] + p[3]);
+    }
+    return d;
+}
+// it takes the place of the tiles' value z, in the sum S as well: a label that is most of S has to cancel
+__device__ __forceinline__ void ce_refine(float cref, float& S, float& z, float better) {
+    const float d = z - better;
+    if (fabsf(d) < 0.5f) {                                    // finite, both of them
+        S -= __builtin_amdgcn_exp2f(fmaf(better, CE_LOG2E, -cref)) * expm1f(d);
+        z = better;
+    }
 }
 
 // (reference, sum) of a row's tiles: running maximum and sum, entries with sum 0 (no class) left out
@@ -264,7 +297,7 @@ struct CeSum {
 
 template <bool GRAD, int NTHR>
 __global__ __launch_bounds__(NTHR) void ce_rows_kernel(const CeRowsArgs a) {
-    __shared__ float red[NTHR / 64][3];
+    __shared__ float red[NTHR / 64][4];
     const int r = blockIdx.x, tid = threadIdx.x;
     if (GRAD && r == 0)
         for (int i = a.N + tid; i < a.g2_pitch; i += NTHR) a.g2[i] = a.g2[a.g2_pitch + i] = 0;
@@ -283,18 +316,26 @@ __global__ __launch_bounds__(NTHR) void ce_rows_kernel(const CeRowsArgs a) {
         return;
     }
     const float2* st = a.stats + (long)r * a.nst;
+    float dot = ce_label_dot(a, r, lab, tid, NTHR), zt = a.zt[r];
     CeSum t = {-INFINITY, 0.f, INFINITY};
     for (int i = tid; i < a.nst; i += NTHR) {
         const float2 v = st[i];
         t.add(v.x, v.y, v.x);
     }
     t.wave();
-    if ((tid & 63) == 0) { red[tid >> 6][0] = t.c; red[tid >> 6][1] = t.s; red[tid >> 6][2] = t.lo; }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+    if ((tid & 63) == 0) { red[tid >> 6][0] = t.c; red[tid >> 6][1] = t.s; red[tid >> 6][2] = t.lo; red[tid >> 6][3] = dot; }
     __syncthreads();
     t = {red[0][0], red[0][1], red[0][2]};
-    for (int w = 1; w < NTHR / 64; ++w) t.add(red[w][0], red[w][1], red[w][2]);
-    const float cref = t.s == 0.f ? 0.f : t.c, S = t.s;       // no class left: S = 0
-    const float zt = a.zt[r];
+    dot = red[0][3];
+    for (int w = 1; w < NTHR / 64; ++w) {
+        t.add(red[w][0], red[w][1], red[w][2]);
+        dot += red[w][3];
+    }
+    const float cref = t.s == 0.f ? 0.f : t.c;                // no class left: S = 0
+    float S = t.s;
+    ce_refine(cref, S, zt, a.bias ? dot + a.bias[lab] : dot);
     const float loss = ce_row_loss(cref, S, zt);
     if (tid == 0) {
         a.rows[r] = loss;
@@ -370,13 +411,18 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
         float v = lab < 0 ? 0.f : NAN;
         if ((unsigned long)lab < (unsigned long)a.V) {
             const float2* st = a.stats + (long)r * a.nst;
+            float dot = ce_label_dot(a, r, lab, lane, 64), zt = a.zt[r];
             CeSum t = {-INFINITY, 0.f, INFINITY};
             for (int i = lane; i < a.nst; i += 64) {
                 const float2 p = st[i];
                 t.add(p.x, p.y, p.x);
             }
             t.wave();
-            v = ce_row_loss(t.s == 0.f ? 0.f : t.c, t.s, a.zt[r]);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+            const float cref = t.s == 0.f ? 0.f : t.c;
+            ce_refine(cref, t.s, zt, a.bias ? dot + a.bias[lab] : dot);
+            v = ce_row_loss(cref, t.s, zt);
         }
         if (lane == 0) a.rows[r] = v;
     }
@@ -1150,6 +1196,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
 
         CeRowsArgs b;
         b.stats = a.stats; b.nst = p.nst; b.wave_cols = p.wave_cols; b.zt = zt; b.labels = a.labels; b.count = count;
+        b.w = w; b.bias = bias;
         b.N = n; b.V = V; b.K = K; b.Vp = p.Vp; b.E = E; b.x = a.x.p; b.xs = xs; b.rows = rows + r0;
         b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch; b.loss = nullptr;
         const bool wide = n <= 256 && p.nst > 512;            // few long rows: 1024 threads each (16 -> 6 us at 4096 entries)

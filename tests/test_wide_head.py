@@ -469,3 +469,18 @@ def test_lowest_value_switches_a_class_off(N, V):
     low = torch.where(torch.isfinite(b), b, torch.full_like(b, torch.finfo(torch.float32).min))
     for p, q in zip(F.dense_softmax_ce(*cuda(x, w, b, lab)), F.dense_softmax_ce(*cuda(x, w, low, lab))):
         assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,V", [(9, 1960, 156), (40, 4096, 500)])
+def test_row_losses_are_not_the_long_sums_error(N, K, V):
+    """The label's logit has the error of a tree of additions (log2 K + 6 of them, the logit and the logarithm rounded at their own
+    size) instead of a chain's; the other classes' errors enter the logarithm by their probabilities, which average them: a
+    quarter of the chain's bound."""
+    x, w, b, lab = make(N, K, V, seed=K)
+    ref = exact(x, w, b, lab)
+    az = (x.double().abs() * w[lab].double().abs()).sum(1) + b[lab].abs().double()
+    own = (math.log2(K) + 6) * U32 * az + 2.0 ** -21 * (1 + ref["rows"].abs())
+    out = F.dense_softmax_ce(*cuda(x, w, b, lab), want_grad=False)
+    err = (out[4].double().cpu() - ref["rows"]).abs()
+    assert (err <= own + ref["t_rows"] / 8).all(), f"{float((err / (own + ref['t_rows'] / 8)).max()):.3g} of its bound"
