@@ -63,7 +63,14 @@ __device__ __forceinline__ void ce_rank(const CeLogitsArgs& a, char* smem, int b
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (b == 0 && a.count) {
         int c = 0;
-        for (int i = tid; i < a.n_all; i += NTHR) c += a.labels_all[i] >= 0;
+        constexpr int U = 8;                                  // loads in flight
+        for (int i = tid; i < a.n_all; i += NTHR * U) {
+            long l[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) l[u] = a.labels_all[min(i + u * NTHR, a.n_all - 1)];
+#pragma unroll
+            for (int u = 0; u < U; ++u) c += l[u] >= 0 && i + u * NTHR < a.n_all;
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
         int* red = (int*)smem;
@@ -79,9 +86,14 @@ __device__ __forceinline__ void ce_rank(const CeLogitsArgs& a, char* smem, int b
     const int r0 = b * CE_RANK_ROWS;
     if (!a.order || r0 >= a.N) return;
     int* lab = (int*)smem;                                   // CE_MAX_ROWS entries at most: 32 KiB
-    for (int i = tid; i < a.N; i += NTHR) {
-        const long l = a.labels[i];
-        lab[i] = (unsigned long)l < (unsigned long)a.V ? (int)l : 0x7fffffff;
+    constexpr int U = 8;
+    for (int i = tid; i < a.N; i += NTHR * U) {
+        long l[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) l[u] = a.labels[min(i + u * NTHR, a.N - 1)];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * NTHR < a.N) lab[i + u * NTHR] = (unsigned long)l[u] < (unsigned long)a.V ? (int)l[u] : 0x7fffffff;
     }
     __syncthreads();
     constexpr int PER = CE_RANK_ROWS / (NTHR / 64);           // rows of a wave, all compared with a label read once
@@ -1199,7 +1211,8 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         b.w = w; b.bias = bias;
         b.N = n; b.V = V; b.K = K; b.Vp = p.Vp; b.E = E; b.x = a.x.p; b.xs = xs; b.rows = rows + r0;
         b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch; b.loss = nullptr;
-        const bool wide = n <= 256 && p.nst > 512;            // few long rows: 1024 threads each (16 -> 6 us at 4096 entries)
+        // few long rows: 1024 threads each (16 -> 6 us at 4096 entries); many short ones: a wave
+        const bool wide = n <= 256 && p.nst > 512, narrow = n > 256 && K <= 512 && p.nst <= 128;
         if (!train) {
             if (N <= CE_FEW_ROWS && p.nst <= CE_FEW_STATS) {
                 ce_score_few_kernel<<<1, 1024, 0, s>>>(b, loss);
@@ -1207,12 +1220,14 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
             }
             if (N == 1) b.loss = loss;
             if (wide) ce_rows_kernel<false, 1024><<<n, 1024, 0, s>>>(b);
+            else if (narrow) ce_rows_kernel<false, 64><<<n, 64, 0, s>>>(b);
             else ce_rows_kernel<false, 256><<<n, 256, 0, s>>>(b);
             if (last && N > 1) ce_mean_kernel<<<1, 1024, 0, s>>>(rows, count, N, loss);
             if (int e = gt_launched()) return e;
             continue;
         }
         if (wide) ce_rows_kernel<true, 1024><<<n, 1024, 0, s>>>(b);
+        else if (narrow) ce_rows_kernel<true, 64><<<n, 64, 0, s>>>(b);
         else ce_rows_kernel<true, 256><<<n, 256, 0, s>>>(b);
 
         CeLabelsArgs l;
