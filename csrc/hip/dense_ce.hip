@@ -50,7 +50,7 @@ struct CeLogitsArgs {
     float* zt;                       // [N] logit of the label
     const long* labels_all; int n_all; float* count;      // block 0 counts the labelled rows of the whole batch
     int* order;                      // [N] rows sorted by (label, row), unlabelled ones last (training)
-    int* slot;                       // [V] reset to -1 (training)
+    int2* slot;                      // [V] reset to -1 (training)
     int nrank;                       // blocks in front of the tiles that do the counting and ranking (a multiple of 8)
     GtMap map;
 };
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 1)) void ce_l
     const int v0 = ta * BA, r0 = tb * BB;
     if (STORE && tb == 0)
         for (int i = tid; i < BA; i += T::NTHR)
-            if (v0 + i < a.V) a.slot[v0 + i] = -1;
+            if (v0 + i < a.V) a.slot[v0 + i] = make_int2(-1, -1);
     // the tile's biases (in powers of two; no class there: -inf, E = 0) and labels, one of each per thread: fetched here, their
     // latency is the loop's, and handed round through LDS behind it (read where they are used: 512 x 1024 x 50021 71 us, 66 so,
     // 2048 x 512 x 32000 99 and 87; all of a lane's own in registers across the loop: 74 and 101)
@@ -445,13 +445,13 @@ __global__ __launch_bounds__(1024) void ce_score_few_kernel(const CeRowsArgs a, 
 
 // ------------------------------------------------------------------------------------------------ 3. label terms
 // Rows in sorted order, in windows of 64 positions: the rows of one class inside a window are a run; its first position i
-// sums it (ascending) into L[i], and next[i] is the window where the class goes on, or -1.  slot[class] is its first run.
+// sums it (ascending) into L[i].  slot[class] holds its first and its last run; those between start at the windows'.
 // Windows bound a block's work whatever the labels are (8000 rows, 1000 of them of one class: 340 us with a block per class,
 // 20 so).  256 threads.  Block 0, in front of them all, takes the mean of the row losses.
 #define CE_RUN 64
 struct CeLabelsArgs {
     const CeRow* row; const int* order; const bf16_t* x; const bf16_t* xs; int N, K;
-    int* slot; int* next; float* L; float* Lb;               // [V], [N], [N][K], [N]
+    int2* slot; float* L; float* Lb;                         // [V], [N][K], [N]
     const float* rows_all; const float* count; int n_all; float* loss;      // loss nullptr: not the last piece
 };
 
@@ -522,9 +522,9 @@ __device__ __forceinline__ void ce_labels(const CeLabelsArgs& a, int i, int chun
         *(float4*)(o + 4) = make_float4(s[4], s[5], s[6], s[7]);
     }
     if (chunk == 0 && tid == 0) {
-        if (fresh) a.slot[lab] = i;
+        if (fresh) a.slot[lab].x = i;
         a.Lb[i] = b;
-        a.next[i] = end < a.N && a.row[a.order[end]].label == lab ? end : -1;
+        if (end >= a.N || a.row[a.order[end]].label != lab) a.slot[lab].y = i;
     }
 }
 __global__ __launch_bounds__(256) void ce_labels_kernel(const CeLabelsArgs a) {
@@ -627,7 +627,7 @@ struct CeDwArgs {
     GtOperand xs, e;                 // column order over the rows: x' [N][K] (columns K), E [N][Vp] (columns Vp)
     int N, V, K;
     const bf16_t* g2; int g2_pitch;  // zero behind row N up to a multiple of 64
-    const int* slot; const int* next; const float* L; const float* Lb;      // the label terms' remainders (ce_labels)
+    const int2* slot; const float* L; const float* Lb;       // the label terms' remainders (ce_labels)
     const float* acc_w; const float* acc_b;       // earlier row pieces ([V][K], [V]) or nullptr
     void* dw; void* db; int out_bf16;             // this piece's output: fp32 (possibly the accumulator) or bf16
     // blocks nv, nv + 1, .. (of the first row of the grid; of 256 threads) finish the splits of dx
@@ -638,16 +638,29 @@ struct CeDwArgs {
     GtMap map;
 };
 
-// what the label terms add to four features / the bias of a class: its runs in order (sl: the first, -1: none)
-__device__ __forceinline__ void ce_label_add(const CeDwArgs& a, int sl, int k, f32x4& d) {
-    for (; sl >= 0; sl = a.next[sl]) {
-        const float4 p = *(const float4*)(a.L + (long)sl * a.K + k);
-        d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
+// what the label terms add to four features / the bias of a class: its runs in order (x the first, -1: none; y the last)
+__device__ __forceinline__ int ce_run_next(int p) { return (p / CE_RUN + 1) * CE_RUN; }
+__device__ __forceinline__ void ce_label_add(const CeDwArgs& a, int2 run, int k, f32x4& d) {
+    if (run.x < 0) return;
+    for (int p = run.x; p <= run.y;) {                        // four loads in flight
+        f32x4 v[4];
+        bool in[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            in[u] = p <= run.y;
+            v[u] = *(const f32x4*)(a.L + (long)min(p, run.y) * a.K + k);
+            p = ce_run_next(p);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] += in[u] ? v[u][e] : 0.f;
     }
 }
-__device__ __forceinline__ float ce_label_bias(const CeDwArgs& a, int sl) {
+__device__ __forceinline__ float ce_label_bias(const CeDwArgs& a, int2 run) {
     float s = 0.f;
-    for (; sl >= 0; sl = a.next[sl]) s += a.Lb[sl];
+    if (run.x >= 0)
+        for (int p = run.x; p <= run.y; p = ce_run_next(p)) s += a.Lb[p];
     return s;
 }
 
@@ -668,25 +681,24 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 3)) void ce_d
     const bool do_db = ta == 0 && wa == 0;                     // wave-uniform
     f32x4 acc[T::NA][T::NB], bacc = {0.f, 0.f, 0.f, 0.f};
     static_assert(T::NB <= 4, "rows of the bias accumulator");
-    int slots[T::NB];                                          // the classes' first label runs
+    int2 slots[T::NB];                                         // the classes' label runs
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int v = v0 + wb * (BB / WB) + 16 * j + fr;
-        slots[j] = v < a.V && !a.rslab ? a.slot[v] : -1;
+        slots[j] = v < a.V && !a.rslab ? a.slot[v] : make_int2(-1, -1);
     }
     const int wk = k0 + wa * (BA / WA) + 4 * fq, wv = v0 + wb * (BB / WB) + fr;
     // The sums start from the label terms, loaded while the first steps are on their way: behind the loop the loads of 16
     // classes at a time waited for each other (2048 x 2048 x 32000: 304 us, 276 so; 512 x 1024 x 50021 82 and 77)
     auto labels = [&](f32x4 (&c)[T::NA][T::NB]) {
-        int any = -1, next[T::NB];
+        int any = -1;
 #pragma unroll
-        for (int j = 0; j < T::NB; ++j) any = max(any, slots[j]);
+        for (int j = 0; j < T::NB; ++j) any = max(any, slots[j].x);
         if (!__any(any >= 0)) return T::clear(c);
         auto at = [&](int sl, int i) { return *(const f32x4*)(a.L + (long)sl * a.K + min(wk + 16 * i, a.K - 4)); };
 #pragma unroll
         for (int j = 0; j < T::NB; ++j) {
-            const int sl = max(slots[j], 0);                  // loaded whether there is one or not, and dropped
-            next[j] = a.next[sl];
+            const int sl = max(slots[j].x, 0);                // loaded whether there is one or not, and dropped
 #pragma unroll
             for (int i = 0; i < T::NA; ++i) c[i][j] = at(sl, i);
         }
@@ -695,11 +707,12 @@ __global__ __launch_bounds__(64 * WA * WB, (BA * BB >= 65536 ? 2 : 3)) void ce_d
 #pragma unroll
             for (int i = 0; i < T::NA; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[i][j][e] = slots[j] >= 0 ? c[i][j][e] : 0.f;
-            for (int sl = slots[j] >= 0 ? next[j] : -1; __any(sl >= 0); sl = sl >= 0 ? a.next[sl] : -1)
+                for (int e = 0; e < 4; ++e) c[i][j][e] = slots[j].x >= 0 ? c[i][j][e] : 0.f;
+            const int last = slots[j].x >= 0 ? slots[j].y : -1;
+            for (int p = ce_run_next(max(slots[j].x, 0)); __any(p <= last); p += CE_RUN)
 #pragma unroll
                 for (int i = 0; i < T::NA; ++i)
-                    if (sl >= 0) c[i][j] += at(sl, i);
+                    if (p <= last) c[i][j] += at(p, i);
         }
     };
     // db = E^T g: one more matrix instruction per B fragment j, against a fragment whose rows 4 j and 4 j + 1 are g's two
@@ -832,9 +845,9 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
     SE se;
     se.init(a.e, v0, 0, a.N, wave, lane);
     se.issue(lds0, wave);
-    int slots[2];
+    int slots[2];                                             // one window: a class has one run
 #pragma unroll
-    for (int j = 0; j < 2; ++j) slots[j] = wv + 16 * j + fr < a.V ? a.slot[wv + 16 * j + fr] : -1;
+    for (int j = 0; j < 2; ++j) slots[j] = wv + 16 * j + fr < a.V ? a.slot[wv + 16 * j + fr].x : -1;
     auto fetch = [&](int k, int buf) {
         SX sx;
         sx.init(a.xs, k, 0, a.N, wave, lane);
@@ -869,7 +882,8 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
         }
         const int v = wv + 16 * fq + fr;
         if (fq < 2 && v < a.V) {
-            float t = b[0] + b[1] + ce_label_bias(a, fq == 0 ? slots[0] : slots[1]);
+            const int sl = fq == 0 ? slots[0] : slots[1];
+            float t = b[0] + b[1] + (sl >= 0 ? a.Lb[sl] : 0.f);
             if (a.acc_b) t += a.acc_b[v];
             if (BF16) ((bf16_t*)a.db)[v] = f2bf(t);
             else ((float*)a.db)[v] = t;
@@ -902,7 +916,7 @@ __global__ __launch_bounds__(256, 3) void ce_dw_thin_kernel(const CeDwArgs a) {
             for (int i = 0; i < 4; ++i) {
                 const int k = c * KC + 16 * i + 4 * fq;
                 f32x4 d = acc[i][j];
-                if (k < a.K) ce_label_add(a, slots[j], k, d);
+                if (k < a.K && slots[j] >= 0) d += *(const f32x4*)(a.L + (long)slots[j] * a.K + k);
                 if (a.acc_w && v < a.V && k < a.K) {
                     const float4 p = *(const float4*)(a.acc_w + (long)v * a.K + k);
                     d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
@@ -979,7 +993,7 @@ struct CePlan {
     int Vp, lt, nst, wave_cols;      // logits: tile, stats entries per row, classes per entry
     int xt, ns, per;                 // dx: tile, splits over the classes, classes per split
     int wt, rs, rper;                // dw: tile, splits over the rows, rows per split
-    long o_count, o_zt, o_stats, o_row, o_order, o_slot, o_next, o_g2, o_xs, o_L, o_Lb, o_E, o_slab, o_rslab, o_accw, o_accb, bytes;
+    long o_count, o_zt, o_stats, o_row, o_order, o_slot, o_g2, o_xs, o_L, o_Lb, o_E, o_slab, o_rslab, o_accw, o_accb, bytes;
     int g2_pitch;
 };
 
@@ -1071,9 +1085,9 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
     long o = 0;
     auto take = [&](long bytes) { const long at = o; o += (bytes + 255) / 256 * 256; return at; };
     p.o_count = take(4); p.o_zt = take(4L * p.R); p.o_stats = take(8L * p.R * p.nst);
-    p.o_row = p.o_order = p.o_slot = p.o_next = p.o_g2 = p.o_xs = p.o_L = p.o_Lb = p.o_E = p.o_slab = p.o_rslab = p.o_accw = p.o_accb = 0;
+    p.o_row = p.o_order = p.o_slot = p.o_g2 = p.o_xs = p.o_L = p.o_Lb = p.o_E = p.o_slab = p.o_rslab = p.o_accw = p.o_accb = 0;
     if (train) {
-        p.o_row = take(32L * p.R); p.o_order = take(4L * p.R); p.o_slot = take(4L * V); p.o_next = take(4L * p.R); p.o_g2 = take(4L * p.g2_pitch);
+        p.o_row = take(32L * p.R); p.o_order = take(4L * p.R); p.o_slot = take(8L * V); p.o_g2 = take(4L * p.g2_pitch);
         p.o_xs = take(2L * p.R * K); p.o_L = take(4L * p.R * K); p.o_Lb = take(4L * p.R); p.o_E = take(2L * p.R * p.Vp);
         if (p.ns > 1) p.o_slab = take(4L * p.ns * p.R * K);
         if (p.rs > 1) p.o_rslab = take(4L * p.rs * V * (K + 1L));
@@ -1202,7 +1216,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         a.bias = bias; a.labels = labels + r0; a.N = n; a.V = V; a.K = K; a.Vp = p.Vp;
         a.E = train ? E : nullptr; a.stats = (float2*)(ws + p.o_stats); a.nst = p.nst; a.zt = zt;
         a.labels_all = labels; a.n_all = N; a.count = r0 == 0 ? count : nullptr;
-        a.order = train ? (int*)(ws + p.o_order) : nullptr; a.slot = (int*)(ws + p.o_slot);
+        a.order = train ? (int*)(ws + p.o_order) : nullptr; a.slot = (int2*)(ws + p.o_slot);
         int rc = train ? ce_logits<true>(a, p.lt, s) : ce_logits<false>(a, p.lt, s);
         if (rc) return rc;
 
@@ -1231,7 +1245,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         else ce_rows_kernel<true, 256><<<n, 256, 0, s>>>(b);
 
         CeLabelsArgs l;
-        l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot; l.next = (int*)(ws + p.o_next);
+        l.row = row; l.order = a.order; l.x = a.x.p; l.xs = xs; l.N = n; l.K = K; l.slot = a.slot;
         l.L = (float*)(ws + p.o_L); l.Lb = (float*)(ws + p.o_Lb);
         l.rows_all = rows; l.count = count; l.n_all = N; l.loss = last ? loss : nullptr;
         if (int e = gt_launched()) return e;
@@ -1253,7 +1267,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         c.rsplit = ce_cdiv(n, p.rper); c.rper = p.rper;     // a shorter last piece has fewer splits
         c.rslab = c.rsplit > 1 ? (float*)(ws + p.o_rslab) : nullptr;
         c.slab = d.slab; c.row = row; c.w = w; c.dx = d.dx; c.nsplit = p.ns; c.nv = 0;
-        c.N = n; c.V = V; c.K = K; c.g2 = g2; c.g2_pitch = p.g2_pitch; c.slot = a.slot; c.next = l.next; c.L = l.L; c.Lb = l.Lb;
+        c.N = n; c.V = V; c.K = K; c.g2 = g2; c.g2_pitch = p.g2_pitch; c.slot = a.slot; c.L = l.L; c.Lb = l.Lb;
         // several pieces add up in fp32: in the output itself, or in the workspace until the last piece rounds
         float* aw = out_bf16 ? (float*)(ws + p.o_accw) : (float*)dw;
         float* ab = out_bf16 ? (float*)(ws + p.o_accb) : (float*)db;
