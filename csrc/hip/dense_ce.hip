@@ -1225,7 +1225,7 @@ DDL_API int ddl_dense_ce(const void* x_, const void* w_, const float* bias, cons
         b.w = w; b.bias = bias;
         b.N = n; b.V = V; b.K = K; b.Vp = p.Vp; b.E = E; b.x = a.x.p; b.xs = xs; b.rows = rows + r0;
         b.row = row; b.g2 = g2; b.g2_pitch = p.g2_pitch; b.loss = nullptr;
-        // few long rows: 1024 threads each (16 -> 6 us at 4096 entries); many short ones: a wave
+        // few long rows: 1024 threads each (16 -> 6 us at 4096 entries); many short ones: a wave (8000 x 64 x 65: 80 -> 72 us)
         const bool wide = n <= 256 && p.nst > 512, narrow = n > 256 && K <= 512 && p.nst <= 128;
         if (!train) {
             if (N <= CE_FEW_ROWS && p.nst <= CE_FEW_STATS) {
