@@ -19,7 +19,7 @@ import torch
 own = False
 
 BLOCK = 32            # elements that share one scale
-MIN_EXP, MAX_EXP = -119, 121      # range of the scale exponents (127 * 2^121 is the largest finite value)
+MIN_EXP = -119        # smallest scale exponent
 EXP_BIAS = 127        # scales are stored as exponent + EXP_BIAS; 255 marks a block that held a NaN or an infinity
 
 
@@ -141,7 +141,7 @@ def _pow2(e):
 
 def _pack_plain(x):
     """(codes int8 like x, scales uint8 [ceil(numel / 32)]): per 32 elements in memory order the smallest power of two
-    s = 2^e, -119 <= e <= 121, with max |x| <= 127 s; code = round-to-even(x / s), but never 0 for an x that is not 0 (the sign survives)."""
+    s with max |x| <= 127 s; code = round-to-even(x / s), but never 0 for an x that is not 0 (the sign survives)."""
     flat = x.reshape(-1).float()
     n = flat.numel()
     nb = (n + BLOCK - 1) // BLOCK
@@ -149,9 +149,9 @@ def _pack_plain(x):
     bad = ~torch.isfinite(blk).all(1)
     blk = torch.where(bad[:, None], torch.zeros_like(blk), blk)
     mant, exp = torch.frexp(blk.abs().amax(1))                 # amax = mant 2^exp, 0.5 <= mant < 1
-    e = (torch.where(mant * 128 <= 127, exp - 7, exp - 6)).clamp(MIN_EXP, MAX_EXP)
+    e = (torch.where(mant * 128 <= 127, exp - 7, exp - 6)).clamp_min(MIN_EXP)
     e = torch.where(mant == 0, torch.full_like(e, MIN_EXP), e)
-    q = torch.round(blk * _pow2(-e)[:, None]).clamp(-127, 127)
+    q = torch.round(blk * _pow2(-e)[:, None])
     q = torch.where((q == 0) & (blk != 0), torch.sign(blk), q)
     codes = q.reshape(-1)[:n].to(torch.int8).view(x.shape)
     scales = torch.where(bad, torch.full_like(e, 255), e + EXP_BIAS).to(torch.uint8)
@@ -290,12 +290,12 @@ def _exact_keep(x):
         top = blk.abs().max(1).values
         e = torch.full_like(top, float(MIN_EXP))
         live = top > 0
-        e[live] = torch.ceil(torch.log2(top[live] / 127)).clamp(MIN_EXP, MAX_EXP)
+        e[live] = torch.ceil(torch.log2(top[live] / 127)).clamp_min(MIN_EXP)
         # the logarithm rounds: settle the exponent by the comparison that defines it
-        e = torch.where((e < MAX_EXP) & (top > 127 * _two_to(e)), e + 1, e)
+        e = torch.where(top > 127 * _two_to(e), e + 1, e)
         e = torch.where((e > MIN_EXP) & (top <= 127 * _two_to(e - 1)), e - 1, e)
         s = _two_to(e)[:, None]
-        q = torch.round(blk / s).clamp(-127, 127)
+        q = torch.round(blk / s)
         q = torch.where((q == 0) & (blk != 0), torch.sign(blk), q)
         val = q * s
         val[~torch.isfinite(blk).all(1)] = math.nan
