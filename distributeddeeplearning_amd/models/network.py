@@ -483,10 +483,8 @@ class ConvOp(Op):
                 dy = F.act_bwd(dy, self.y, self.act, self.alpha)
         x = self.x
         dx = None
-        if isinstance(x, F.Packed8):
-            if self.kind == "dense":
-                return self._bwd_dense8(x, dy, need_dx, need_dw, mul)
-            x = F.unpack8(x) if need_dw else x
+        if isinstance(x, F.Packed8) and self.kind == "dense":
+            return self._bwd_dense8(x, dy, need_dx, need_dw, mul)
         if self.onech == "up" or (self.stream1 and self.stream_used):
             bnd, self.bn_deferred = self.bn_deferred, None
             if need_dw and not need_dx and self.x_affine is None:
@@ -529,7 +527,9 @@ class ConvOp(Op):
             # core X = our output (dy), core Y = our input (x)
             if need_dw:
                 def wg():
-                    xx = x
+                    # a checkpoint is unpacked here and not above: on the branch the tensor belongs to the branch's
+                    # stream, so its memory cannot go to a later main-stream tensor while the branch reads it
+                    xx = _saved(x)
                     if self.x_affine is not None:       # the BatchNorm output was never written
                         sc, sh, groups, ctrue = self.x_affine
                         hip = F.hip_backend()
@@ -562,7 +562,7 @@ class ConvOp(Op):
                 dx = self._dw_bn_bwd(dy, need_dw)
             if need_dw:
                 def wg():
-                    xx, xa = x, None
+                    xx, xa = _saved(x), None            # (unpacked on the branch, as above)
                     if self.x_affine is not None:       # depthwise behind a BatchNorm applied on load
                         sc, sh, groups, ctrue = self.x_affine
                         if g.depthwise and groups == 1:

@@ -1,0 +1,110 @@
+"""Whole training steps of networks that keep their activations in 8 bits: which memory the weight-gradient branch reads, what
+is still held in bf16, and captured steps against eager ones."""
+import weakref
+
+import pytest
+import torch
+
+from distributeddeeplearning_amd import config
+from distributeddeeplearning_amd.models import ir, network, search
+from distributeddeeplearning_amd.models.classifier import RandomModel
+from distributeddeeplearning_amd.models.network import Network
+from distributeddeeplearning_amd.models.optim import OptimConfig
+from distributeddeeplearning_amd.ops import functional as F
+from distributeddeeplearning_amd.utils.data import Data
+
+
+def spec(*layers, shape=(8, 8, 4)):
+    m = ir.ModelSpec("m", [ir.Input("in", shape)])
+    for l in layers:
+        m.append(l)
+    return m
+
+
+def conv_net(shape=(8, 8, 4)):
+    """Every convolution of the general path that keeps its input in 8 bits, with and without a BatchNorm behind it."""
+    return spec(ir.Conv2D("c0", 16, (3, 3), 1, 1, "same", "relu"), ir.BatchNorm("b0"),
+                ir.Conv2D("c1", 24, (3, 3), 1, 1, "same", "tanh"), ir.BatchNorm("b1"),
+                ir.Conv2DTranspose("t1", 16, (3, 3), 2, 1, "same", "relu"), ir.BatchNorm("b2"),
+                ir.Conv2D("c2", 16, (3, 3), 2, 1, "same", "relu"), ir.DepthwiseConv2D("w1", (3, 3), 1, 1, "same", "relu"),
+                ir.Conv2D("c3", 16, (3, 3), 2, 1, "same", "relu"),
+                ir.Flatten("f"), ir.Dense("d1", 24, "relu"), ir.Dense("o", 10, "softmax"), shape=shape)
+
+
+def images(n, seed=0, shape=(8, 8, 4)):
+    g = torch.Generator().manual_seed(seed)
+    return torch.rand(n, *shape, generator=g).bfloat16().float()
+
+
+def grads(net):
+    return {(p.layer, p.wname): net.G[p.offset:p.offset + p.numel].view(p.shape)[p.corner()].float().cpu().clone()
+            for p in net.param_table() if p.trainable}
+
+
+# ------------------------------------------------------------------------------------------------ the weight-gradient branch
+def test_branch_reads_only_what_is_held_until_the_join(monkeypatch):
+    """What the branch reads from outside it is still referenced when it is joined (a checkpoint unpacked on the main stream and
+    dropped there could be overwritten under the branch's kernel)."""
+    inside, read, made, checked = [], [], set(), []
+    wgrad, unpack = F.conv_wgrad, F.unpack8
+    kept = []
+
+    def branch(fn, *keep):
+        kept.extend(keep)
+        inside.append(1)
+        fn()
+        inside.pop()
+        made.clear()
+
+    def spy_wgrad(x, dy, *a, **k):
+        for t in (x, dy):
+            if inside and id(t) not in made and t._base is None:
+                read.append(weakref.ref(t))
+        return wgrad(x, dy, *a, **k)
+
+    def spy_unpack(q, out=None):
+        y = unpack(q, out).clone()                 # (a tensor of its own, not a view)
+        if inside:
+            made.add(id(y))
+        return y
+
+    def spy_join():
+        checked.extend(r() is not None for r in read)
+        read.clear()
+        kept.clear()
+    monkeypatch.setattr(network._BR, "run", branch)
+    monkeypatch.setattr(network._BR, "join", spy_join)
+    monkeypatch.setattr(F, "conv_wgrad", spy_wgrad)
+    monkeypatch.setattr(F, "unpack8", spy_unpack)
+    net = Network(conv_net(), "cpu", seed=1)
+    net.keep8 = True
+    y = net.forward(net.prepare_input(images(4)), training=True)
+    assert any(isinstance(op.x, F.Packed8) and op.kind != "dense" for op in net.ops if isinstance(op, network.ConvOp))
+    net.backward(torch.ones_like(y))
+    assert len(checked) >= 5 and all(checked)
+
+
+def member(data, m, over, use_graph, seed=0):
+    sp = config.get_space("ddl_ray", ["data_train_size=1200", *over])
+    cs = search.CompiledSpec(m, OptimConfig.keras("adam", 1e-3), "categorical_crossentropy")
+    return RandomModel(data, data.get_random_sample(1200, seed=seed), sp, cs, "cuda", 0, seed=seed, verbose=False,
+                       use_graph=use_graph)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [32, 128, 200])
+def test_captured_convolution_steps_equal_eager_steps(batch):
+    """Batches of 128 and more issue the weight gradients on the side branch (RandomModel); each replay against an eager step,
+    with eager work between the replays."""
+    data = Data("cuda", channels=3, n_train=1400, n_test=40, synthetic=True)
+    m = conv_net(data.input_shape)
+    a, b = (member(data, m, ["keep8=1", f"batch_size={batch}"], g) for g in (False, True))
+    assert a.net.branch_wgrad == b.net.branch_wgrad == (batch >= 128)
+    idx = a.sample.train_idx
+    for i in range(5):
+        part = idx[i * batch:(i + 1) * batch]
+        la, lb = a.train_step(part), b.train_step(part)
+        torch.cuda.synchronize()
+        assert torch.equal(la, lb), i
+        assert torch.equal(a.net.P, b.net.P) and torch.equal(a.net.S, b.net.S), i
+        b.predict(data.test_x)
