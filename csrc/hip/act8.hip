@@ -194,7 +194,9 @@ struct A8Stage {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             code[u] = __builtin_amdgcn_raw_buffer_load_b64(rc, off[u], 0, 0);
-            scale[u] = __builtin_amdgcn_raw_buffer_load_b8(rs, off[u] == GT_OOB ? GT_OOB : off[u] >> 5, 0, 0);
+            // past the last code no scale either: the last block may be a partial one, and marked 255 (NaN) it would reach
+            // the features that its unused rest stands for
+            scale[u] = __builtin_amdgcn_raw_buffer_load_b8(rs, off[u] < (unsigned)n ? off[u] >> 5 : GT_OOB, 0, 0);
         }
         c += GT_BK * ld;
         s += 2 * ld;

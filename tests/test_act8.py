@@ -284,3 +284,20 @@ def test_refusals():
                  lambda: F.dense_wgrad8(q, x.cpu())):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
+@pytest.mark.parametrize("R,K,O,col", [(65, 72, 24, 70), (65, 72, 24, 3), (129, 264, 40, 263), (33, 8, 16, 1), (64, 72, 8, 71)])
+def test_dense_wgrad8_bad_last_block(tile, R, K, O, col, monkeypatch):
+    """R K is no multiple of 32 in most of these, so the last block is a partial one: bad, it reaches the gradients of its own
+    features and of no others, whatever the tile."""
+    from distributeddeeplearning_amd.ops import hip
+    monkeypatch.setattr(hip, "WGRAD8_TILE", tile)
+    x, dy = values(R, K, 1, 0.0), values(R, O, 2, 0.0)
+    x[R - 1, col] = math.inf
+    dw, db = F.dense_wgrad8(F.pack8(x.cuda()), dy.cuda())
+    nan = torch.zeros(R * K, dtype=torch.bool)
+    first = ((R - 1) * K + col) // 32 * 32
+    nan[first:first + 32] = True
+    assert torch.equal(torch.isnan(dw).cpu(), nan.view(R, K).any(0).expand(O, K)) and torch.isfinite(db).all()
