@@ -732,10 +732,11 @@ class BNOp(Op):
         if self.bwd_done:
             self.bwd_done = False
             return dy
-        if isinstance(self.x, F.Packed8) or isinstance(self.y, F.Packed8):
-            self.x, self.y = _saved(self.x), _saved(self.y)
-        if self.y is None and self.post_act in (None, "linear"):
-            self.y = self.x             # not kept (keep8): nothing behind us to differentiate through it
+        # out of their checkpoints for this call only: kept on the op, every BatchNorm that the pass has left behind would hold
+        # its activations in bf16 again
+        x, y = _saved(self.x), _saved(self.y)
+        if y is None and self.post_act in (None, "linear"):
+            y = x                       # not kept (keep8): nothing behind us to differentiate through it
         conv = self.bias_grad_for
         pre, self.pre_bwd = self.pre_bwd, None
         tgt = self.defer_apply_to
@@ -745,21 +746,21 @@ class BNOp(Op):
             # The layer below is the network's first (a Conv2DTranspose from the one-channel image): our dx has exactly
             # one consumer, that layer's weight gradient, which forms it on load from (dy, x) -- the apply pass and the
             # dx tensor (213 MB for model0 at batch 512) are not needed.  Reduction + finalize only here.
-            c1, c2 = F.hip_backend().bn_bwd_sums(dy, self.x, self.mean.reshape(-1), self.invstd.reshape(-1), self.gamma,
+            c1, c2 = F.hip_backend().bn_bwd_sums(dy, x, self.mean.reshape(-1), self.invstd.reshape(-1), self.gamma,
                                                  self.prev_act, self.prev_alpha, self.ggamma, self.gbeta,
                                                  conv.gbias if conv is not None else None)
-            tgt.bn_deferred = dict(x=self.x, mean=self.mean.reshape(-1), invstd=self.invstd.reshape(-1),
+            tgt.bn_deferred = dict(x=x, mean=self.mean.reshape(-1), invstd=self.invstd.reshape(-1),
                                    gamma=self.gamma, c1=c1, c2=c2, act=self.prev_act, alpha=self.prev_alpha)
             return dy
         if pre is not None and pre[2] == (5 if (need_dw and conv is not None) else 2):
             dx, _, _ = F.hip_backend().bn_bwd(
-                dy, self.x, None, self.mean, self.invstd, self.gamma, None, 0.3, self.used_batch_stats, self.prev_act,
+                dy, x, None, self.mean, self.invstd, self.gamma, None, 0.3, self.used_batch_stats, self.prev_act,
                 self.prev_alpha, self.ggamma if need_dw else None, self.gbeta if need_dw else None,
                 conv.gbias if (need_dw and conv is not None) else None, self.groups_used, part=pre[0],
                 part_blocks=pre[1])
             return dx
-        no_y = self.x.is_cuda and (self.y is self.x or self.post_act in (None, "linear"))
-        dx, _, _ = F.bn_bwd(dy, self.x, None if no_y else self.y, self.mean, self.invstd,
+        no_y = x.is_cuda and (y is x or self.post_act in (None, "linear"))
+        dx, _, _ = F.bn_bwd(dy, x, None if no_y else y, self.mean, self.invstd,
                             self.gamma, self.post_act,
                             self.post_alpha, self.used_batch_stats, self.prev_act, self.prev_alpha,
                             self.ggamma if need_dw else None, self.gbeta if need_dw else None,

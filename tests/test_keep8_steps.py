@@ -108,3 +108,48 @@ def test_captured_convolution_steps_equal_eager_steps(batch):
         assert torch.equal(la, lb), i
         assert torch.equal(a.net.P, b.net.P) and torch.equal(a.net.S, b.net.S), i
         b.predict(data.test_x)
+
+
+# ------------------------------------------------------------------------------------------------ what a step holds
+def test_batchnorm_stays_packed_through_the_backward_pass():
+    net = Network(conv_net(), "cpu", seed=1)
+    net.keep8 = True
+    y = net.forward(net.prepare_input(images(4)), training=True)
+    bns = [op for op in net.ops if isinstance(op, network.BNOp)]
+    kept = [op.x for op in bns]
+    assert all(isinstance(t, F.Packed8) for t in kept)
+    net.backward(torch.ones_like(y))
+    assert all(op.x is t and op.y is None for op, t in zip(bns, kept))
+
+
+def peak_of_a_step(m, keep8, batch, shape):
+    """Bytes that a forward and a backward pass take at most beyond what is there before (plans tuned in a first pass)."""
+    net = Network(m, "cuda", 0)
+    net.keep8 = keep8
+    x = net.prepare_input(images(batch, shape=shape))
+    for _ in range(2):
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = net.forward(x, training=True)
+        dy = torch.ones_like(y)
+        del y
+        net.backward(dy)
+        torch.cuda.synchronize()
+        peak = torch.cuda.max_memory_allocated() - base
+        del dy
+        net.release()
+    return peak
+
+
+@pytest.mark.gpu
+def test_keep8_lowers_the_peak_of_a_batchnorm_network():
+    """Per layer two tensors of A bytes are kept (the convolution's input and the BatchNorm's) at 33 / 64 of that.  What comes on
+    top of the bf16 step's own temporaries: one unpacked tensor, an act_bwd8 result, and codes beside the tensor being packed."""
+    layers, shape = 8, (32, 32, 32)
+    m = spec(*[l for i in range(layers) for l in (ir.Conv2D(f"c{i}", 32, (3, 3), 1, 1, "same", "relu"), ir.BatchNorm(f"b{i}"))],
+             ir.Flatten("f"), ir.Dense("o", 10, "softmax"), shape=shape)
+    A = 128 * 32 * 32 * 32 * 2
+    off, on = (peak_of_a_step(m, k, 128, shape) for k in (False, True))
+    print(f"peak {off / A:.2f} A in bf16, {on / A:.2f} A in 8 bits")
+    assert on <= off - (2 * layers - 1) * A * 31 // 64 + 3 * A        # (the first layer's input is the network's: not packed)
