@@ -145,8 +145,8 @@ class Op:
 
     def keep8(self, x, y):
         """After a training forward: keep what the backward pass needs in 8 bits.  `x` / `y` return the op's input and
-        output packed (each packed once, also when two ops keep it).  False: this op's kernels want bf16 -- or the op
-        keeps nothing of its own -- and its output may still be held in bf16."""
+        output packed (each packed once, also when two ops keep it).  False: this op's kernels want bf16, and its input and
+        output may still be held in bf16.  An op that keeps neither (padding, scaling) has nothing to pack and returns True."""
         return False
 
 
@@ -795,6 +795,9 @@ class PadOp(Op):
     def bwd(self, dy, need_dx=True, need_dw=True):
         return F.spatial_pad(dy, -self.pt, -self.pb, -self.pl, -self.pr)
 
+    def keep8(self, x, y):
+        return True
+
 
 class ActOp(Op):
     def __init__(self, spec, act, alpha, c_true):
@@ -830,6 +833,9 @@ class AffineOp(Op):
 
     def bwd(self, dy, need_dx=True, need_dw=True):
         return F.affine(dy, self.scale, 0.0, self.c_true)
+
+    def keep8(self, x, y):
+        return True
 
 
 class _Keep8:
@@ -875,8 +881,8 @@ class Network:
         self.branch_wgrad = False       # captured steps: wgrad chain as a parallel graph branch (SideBranch)
         # Keep the activations between forward and backward in 8 bits (33 bytes per 32 elements instead of 64; half a step
         # of 2^-7 of a block's largest value).  Applies to Dense / Conv2D / Conv2DTranspose / BatchNorm / activation layers
-        # on the general kernels; the input of the network and what the fused one-channel and BatchNorm-on-load kernels read
-        # stay bf16.
+        # on the general kernels, behind padding and scaling layers too; the input of the network (not a padded or scaled copy
+        # of it) and what the fused one-channel and BatchNorm-on-load kernels read stay bf16.
         self.keep8 = False
         # CPU oracle only: round every op's output (forward) and input gradient (backward) to bf16, the points at
         # which the device executor stores bf16 tensors -- the oracle then differs from the device by fp32

@@ -111,6 +111,48 @@ def test_captured_convolution_steps_equal_eager_steps(batch):
 
 
 # ------------------------------------------------------------------------------------------------ what a step holds
+def padded_net(shape=(8, 8, 4)):
+    return spec(ir.ZeroPadding2D("p0", 1), ir.Conv2D("c0", 16, (3, 3), 1, 1, "valid", "relu"), ir.BatchNorm("b0"),
+                ir.ZeroPadding2D("p1", 1), ir.Conv2D("c1", 16, (3, 3), 1, 1, "valid", "relu"), ir.ZeroPadding2D("p2", 2),
+                ir.LambdaAffine("s", 0.5, 0.25), ir.Conv2D("c2", 8, (3, 3), 2, 1, "valid", "tanh"), ir.Flatten("f"),
+                ir.LambdaAffine("s2", 2.0, 0.0), ir.Dense("o", 10, "softmax"), shape=shape)
+
+
+def check_padded(device):
+    """The layers behind a padding or a scaling keep their input in 8 bits, and the backward pass is that of a bf16 network
+    whose kept tensors are what the checkpoints stand for."""
+    a, b = (Network(padded_net(), device, seed=3) for _ in range(2))
+    b.keep8 = True
+    x = images(9)
+    ya, yb = (n.forward(n.prepare_input(x), training=True) for n in (a, b))
+    assert torch.equal(ya, yb)
+    for op, to in zip(b.ops, a.ops):
+        if isinstance(op, (network.ConvOp, network.BNOp)):
+            assert isinstance(op.x, F.Packed8), op.name
+            to.x = F.unpack8(op.x).reshape(to.x.shape).to(to.x.dtype)
+            if op.y is not None:
+                to.y = F.unpack8(op.y).reshape(to.y.shape).to(to.y.dtype)
+    g = torch.Generator().manual_seed(2)
+    dy = torch.zeros(ya.shape)
+    dy[:, :10] = torch.randn(9, 10, generator=g)
+    for n in (a, b):
+        n.backward(dy.to(device=device, dtype=ya.dtype))
+    ga, gb = grads(a), grads(b)
+    # on the device one bf16 rounding of a dY where the input-gradient kernel would have multiplied by act'
+    tol = 1e-5 if device == "cpu" else 2.0 ** -8
+    for k in ga:
+        assert float((gb[k] - ga[k]).norm()) <= tol * float(ga[k].norm()) + 1e-12, k
+
+
+def test_layers_behind_padding_keep_8_bits_cpu():
+    check_padded("cpu")
+
+
+@pytest.mark.gpu
+def test_layers_behind_padding_keep_8_bits():
+    check_padded("cuda")
+
+
 def test_batchnorm_stays_packed_through_the_backward_pass():
     net = Network(conv_net(), "cpu", seed=1)
     net.keep8 = True
