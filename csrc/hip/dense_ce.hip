@@ -986,6 +986,9 @@ DDL_API int ddl_softmax_wide(const void* logits, float* probs, int B, int Cs, in
 
 // ------------------------------------------------------------------------------------------------ host side
 #define CE_MAX_ROWS 8192      // rows of a piece (their labels are ranked in 32 KiB of LDS)
+// A scoring piece: a launch holds less than 2^32 threads; ce_rows takes 256 of them per row, ce_logits 256 per 128 statistics
+#define CE_SCORE_ROWS (1 << 20)
+constexpr long CE_SCORE_STATS = 4L << 30;  // bytes, 8 per row and wave tile
 
 // Everything a call decides from its sizes alone.
 struct CePlan {
@@ -1009,6 +1012,9 @@ static CePlan ce_plan(int N, int V, int K, bool train, bool acc, long budget, in
         r = r >= 256 ? r / 256 * 256 : 64;
         if (r > CE_MAX_ROWS) r = CE_MAX_ROWS;
         if (p.R > r) p.R = (int)r;
+    } else {
+        if (p.R > CE_SCORE_ROWS) p.R = CE_SCORE_ROWS;
+        if (budget > CE_SCORE_STATS) budget = CE_SCORE_STATS;
     }
     // logits: up to 32 rows the tiles that pad them least, the small ones for enough blocks; else by the estimated time, 64-deep
     // steps plus a block's ends in rounds of one 256 x 256 block or two of 128 x 128 or 128 x 32 per CU (the large and the

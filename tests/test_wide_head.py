@@ -151,6 +151,18 @@ def test_cpu_refusals():
         F.dense_softmax_ce(x, w, None, lab, out_db=torch.empty(80))
 
 
+def test_scored_rows_come_in_pieces_a_launch_can_hold():
+    """A piece's launches hold less than 2^32 threads (256 per row, 256 per 128 statistics of 8 bytes), so its workspace stops
+    growing: at 2^20 rows, and at 4 GiB of statistics however much the caller allows."""
+    from distributeddeeplearning_amd.ops import hip
+    for K, V in ((520, 100), (8, 100), (1024, 5000)):
+        most = hip._dense_ce_ws(1 << 20, V, K, 0, 0, 4 << 30, -1)
+        assert 0 < hip._dense_ce_ws(1 << 19, V, K, 0, 0, 4 << 30, -1) < most
+        for n in ((1 << 20) + 1, 1 << 24, (1 << 28) - 1):
+            assert hip._dense_ce_ws(n, V, K, 0, 0, 4 << 30, -1) == most
+    assert hip._dense_ce_ws(1 << 20, 1 << 21, 64, 0, 0, 1 << 40, -1) <= (4 << 30) + (8 << 20)
+
+
 # ------------------------------------------------------------------------------------------------ device
 def cuda(x, w, b, lab):
     return x.cuda(), w.cuda(), None if b is None else b.cuda(), lab.cuda()
@@ -484,3 +496,17 @@ def test_row_losses_are_not_the_long_sums_error(N, K, V):
     out = F.dense_softmax_ce(*cuda(x, w, b, lab), want_grad=False)
     err = (out[4].double().cpu() - ref["rows"]).abs()
     assert (err <= own + ref["t_rows"] / 8).all(), f"{float((err / (own + ref['t_rows'] / 8)).max()):.3g} of its bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [((1 << 24) + 64, 520), ((1 << 26) + 64, 8)])
+def test_scoring_more_rows_than_a_launch_holds(N, K):
+    """Blocks of 256 and of 64 threads per row, 2^32 threads and more over all the rows.  64 rows repeated: each has the bits of
+    its first copy, and those are right."""
+    a = make(64, K, 100, seed=K)
+    x, w, b, lab = cuda(*a)
+    x, lab = (t.expand(N // 64, *t.shape).reshape(N, *t.shape[1:]).contiguous() for t in (x, lab))
+    loss, _, _, _, rows = F.dense_softmax_ce(x, w, b, lab, want_grad=False)
+    ref = exact(*a)
+    check((loss, None, None, None, rows[:64]), ref)
+    assert torch.equal(rows.view(-1, 64), rows[:64].expand(N // 64, 64))
