@@ -980,13 +980,17 @@ __global__ __launch_bounds__(256) void softmax_wide_kernel(const bf16_t* __restr
 
 DDL_API int ddl_softmax_wide(const void* logits, float* probs, int B, int Cs, int N, hipStream_t s) {
     if (B <= 0 || N <= 0 || N > Cs || (Cs & 7)) return -1;
-    softmax_wide_kernel<<<B, 256, 0, s>>>((const bf16_t*)logits, probs, Cs, N);
+    constexpr int ROWS = 1 << 20;                             // per launch: the runtime takes a grid's threads modulo 2^32
+    for (long r = 0; r < B; r += ROWS)
+        softmax_wide_kernel<<<(int)(B - r < ROWS ? B - r : ROWS), 256, 0, s>>>((const bf16_t*)logits + r * Cs,
+                                                                        probs + r * N, Cs, N);
     return gt_launched();
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 #define CE_MAX_ROWS 8192      // rows of a piece (their labels are ranked in 32 KiB of LDS)
-// A scoring piece: a launch holds less than 2^32 threads; ce_rows takes 256 of them per row, ce_logits 256 per 128 statistics
+// A scoring piece: a launch holds less than 2^32 threads (the runtime takes more modulo 2^32, without an error); ce_rows
+// takes 256 of them per row, ce_logits 256 per 128 statistics
 #define CE_SCORE_ROWS (1 << 20)
 constexpr long CE_SCORE_STATS = 4L << 30;  // bytes, 8 per row and wave tile
 

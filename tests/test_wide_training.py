@@ -274,3 +274,17 @@ def test_softmax_of_wide_rows(B, N):
     assert got.shape == ref.shape and ((got - ref).abs() <= 2.0 ** -15 * ref + 1e-30).all()
     with pytest.raises(ValueError):
         F.softmax_ce(z.cuda(), torch.zeros(B, N, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_softmax_of_more_wide_rows_than_a_launch_holds():
+    """2^24 blocks of 256 threads and more are taken modulo 2^32 threads, without an error: 64 rows repeated have the bits of their first copies."""
+    g = torch.Generator().manual_seed(1)
+    z = torch.zeros(64, 72)
+    z[:, :65] = torch.randn(64, 65, generator=g) * 4
+    z = z.bfloat16().cuda()
+    B = (1 << 24) + 64
+    one, all_ = F.softmax(z, 65), F.softmax(z.expand(B // 64, 64, 72).reshape(B, 72), 65)
+    assert torch.equal(all_.view(-1, 64, 65), one.expand(B // 64, 64, 65))
+    ref = torch.softmax(z[:, :65].double(), 1)
+    assert ((one.double() - ref).abs() <= 2.0 ** -15 * ref).all()
