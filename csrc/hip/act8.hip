@@ -391,7 +391,7 @@ static int launch_wgrad8(Wg8Args& a, hipStream_t s) {
     constexpr int lds = 2 * (BA + BB) * GT_BK * 2;
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.O + BB - 1) / BB, a.nsplit, 4);
-    if (!gt_map_ok(a.map)) return -1;
+    if (!gt_map_ok(a.map, 64 * WA * WB)) return -1;
     kern<<<gt_grid(a.map), 64 * WA * WB, lds, s>>>(a);
     return gt_launched();
 }

@@ -1116,8 +1116,8 @@ static int launch_logits(CeLogitsArgs& a, hipStream_t s) {
     constexpr auto kern = ce_logits_kernel<BA, BB, WA, WB, STAGES, STORE>;
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.Vp + BA - 1) / BA, (a.N + BB - 1) / BB, 1, 8);
-    if (!gt_map_ok(a.map)) return -1;
     a.nrank = a.order ? (ce_cdiv(a.N, CE_RANK_ROWS) + 7) / 8 * 8 : 8;
+    if (!gt_map_ok(a.map, T::NTHR, a.nrank)) return -1;
     kern<<<a.nrank + gt_grid(a.map), T::NTHR, lds, s>>>(a);
     return gt_launched();
 }
@@ -1138,7 +1138,7 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     constexpr auto kern = ce_dx_kernel<BA, BB, WA, WB, STAGES>;
     if (int rc = gt_lds<kern>(T::LDS_BYTES)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.N + BB - 1) / BB, a.nsplit, 8);
-    if (!gt_map_ok(a.map)) return -1;
+    if (!gt_map_ok(a.map, T::NTHR, 2048)) return -1;
     a.nlab_chunks = ce_cdiv(a.K, 2048);
     a.ntile = gt_grid(a.map);
     // The label blocks fill what the last round of tiles leaves (a launch of their own costs 5 us; the large tiles have other
@@ -1150,6 +1150,12 @@ static int launch_dx(CeDxArgs& a, hipStream_t s) {
     return gt_launched();
 }
 
+// blocks that finish the splits of dx: four features per thread, and strides of them in a piece of 2^30 features and more
+static int ce_finish_blocks(const CeDwArgs& a) {
+    const long n = a.slab ? ((long)a.N * a.K + 1023) / 1024 : 0;
+    return n < (1 << 20) ? (int)n : 1 << 20;
+}
+
 template <int BA, int BB, int WA, int WB, int STAGES, int BK>
 static int launch_dw(CeDwArgs& a, hipStream_t s) {
     using T = GtTile<BA, BB, WA, WB, true, true, STAGES, GT_PRIO, BK>;
@@ -1158,10 +1164,10 @@ static int launch_dw(CeDwArgs& a, hipStream_t s) {
     const size_t lds = a.out_bf16 && out > T::LDS_BYTES ? out : T::LDS_BYTES;
     if (int rc = gt_lds<kern>(lds)) return rc;
     a.map = gt_make_map((a.K + BA - 1) / BA, (a.V + BB - 1) / BB, a.rsplit, 4);
-    if (!gt_map_ok(a.map)) return -1;
     // the splits of dx are finished in what the last round of tiles leaves, or by a launch of their own (7 us)
     a.nv = gt_grid(a.map);
-    const int nfin = a.slab ? (int)(((long)a.N * a.K + 1023) / 1024) : 0;
+    const int nfin = ce_finish_blocks(a);
+    if (!gt_map_ok(a.map, T::NTHR, nfin)) return -1;
     if (T::NTHR != 256 && nfin) ce_dx_finish_kernel<<<nfin, 256, 0, s>>>(a.slab, a.row, a.w, a.dx, a.N, a.K, a.nsplit);
     kern<<<a.nv + (T::NTHR == 256 ? nfin : 0), T::NTHR, lds, s>>>(a);
     if (a.rsplit > 1) {
@@ -1180,7 +1186,7 @@ static int launch_dw_thin(CeDwArgs& a, hipStream_t s) {
     if (int rc = gt_lds<kern>(lds)) return rc;
     const int nc = (a.K + 63) / 64;
     a.nv = (a.V + 127) / 128;
-    const int want = (768 + a.nv - 1) / a.nv, nfin = a.slab ? ce_cdiv((long)a.N * a.K, 1024) : 0;
+    const int want = (768 + a.nv - 1) / a.nv, nfin = ce_finish_blocks(a);
     kern<<<dim3(a.nv + nfin, want < nc ? want : nc), 256, lds, s>>>(a);
     return gt_launched();
 }

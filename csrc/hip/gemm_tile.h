@@ -271,7 +271,10 @@ static inline GtMap gt_make_map(int na, int nb, int ns, int gb) {
     return m;
 }
 static inline unsigned gt_grid(const GtMap& m) { return (unsigned)(((long)m.na * m.nb * m.ns + 7) / 8 * 8); }
-static inline bool gt_map_ok(const GtMap& m) { return (long)m.na * m.nb * m.ns < (1L << 30); }      // gt_map counts in int
+// gt_map counts in int, and the runtime takes a launch's threads modulo 2^32 without an error; `more`: blocks beside the tiles
+static inline bool gt_map_ok(const GtMap& m, int threads, long more = 0) {
+    return ((long)m.na * m.nb * m.ns + 8 + more) * threads < (1L << 32);
+}
 
 // dynamic LDS above 64 KiB has to be asked for, once per kernel and device
 template <auto Kern>
