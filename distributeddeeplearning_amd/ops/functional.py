@@ -241,6 +241,23 @@ def dense1_bce_fwd_bwd(x, w, b, label_first, label_second, n_first, want_dx=True
     return loss, dx, dw, db, logits
 
 
+def _apart(what, outs, ins):
+    """Refuse outputs that share memory with an input or with one another: kernels write outputs while others still read (a
+    gradient over the bias would be the next piece of rows' bias).  (name, tensor or None) each; contiguous ones, as the device
+    wants them."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+    done = [(n, *span(t)) for n, t in ins if t is not None and t.numel() and t.is_contiguous()]
+    for name, t in outs:
+        if t is None or not t.numel() or not t.is_contiguous():
+            continue
+        lo, hi = span(t)
+        for other, a, b in done:
+            if lo < b and a < hi:
+                raise ValueError(f"{what}: {name} overlaps {other}")
+        done.append((name, lo, hi))
+
+
 def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):
     """Dense(K -> V) + softmax cross entropy for any number of classes, forward and backward, without the logits.
 
@@ -249,11 +266,14 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
     whose label is negative takes no part, whatever its x holds: row loss 0, dx 0, not counted.  Returns (loss, dx, dw, db,
     rows): the mean over the labelled rows (0 if there are none), the gradients of that mean (None without `want_grad`; db
     None without a bias) and the row losses.  dx has x's type, dw [V][K] and db [V] `grad_dtype` (fp32 | bf16), or they
-    overwrite `out_dw` / `out_db` in those tensors' type (out_dw apart from w and x).
+    overwrite `out_dw` / `out_db` in those tensors' type, which share no memory with each other or with an input.
 
     A label past the last class makes its row loss (and the mean) NaN and its row no gradient; a labelled row with a NaN
     or infinite logit, or with every class switched off, has NaN loss and gradients.  On the device the gradient of the
     logits is rounded to bf16 as every dY is, twice for dw (its scale is folded into x)."""
+    if out_dw is not None or out_db is not None:
+        _apart("dense_softmax_ce", (("out_dw", out_dw), ("out_db", out_db)),
+               (("x", x), ("w", w), ("bias", bias), ("labels", labels)))
     if x.is_cuda:
         return hip_backend().dense_softmax_ce(x, w, bias, labels, want_grad, out_dw, out_db, grad_dtype)
     loss, dx, dw, db, rows = cpu_ref.dense_softmax_ce(x, w, bias, labels, want_grad)
@@ -308,7 +328,9 @@ def pack8(x):
 
 
 def unpack8(q, out=None):
-    """Packed8 -> activation tensor (device: bf16, exact; CPU: fp32)."""
+    """Packed8 -> activation tensor (device: bf16, exact; CPU: fp32), into `out` (apart from the checkpoint) if given."""
+    if out is not None:
+        _apart("unpack8", (("out", out),), (("the codes", q.codes), ("the scales", q.scales)))
     return (hip_backend() if q.codes.is_cuda else cpu_ref).unpack8(q, out)
 
 
@@ -325,8 +347,12 @@ def act_bwd8(dy, q, kind, alpha=0.3):
 
 def dense_wgrad8(q, dy, out_dw=None, out_db=None, n_out=None):
     """Gradients of a Dense layer's weights [O][K] and bias [O] (fp32) from its input's 8-bit checkpoint [R][K] and
-    dy [R][Op]; `n_out`: O, when dy carries padding lanes behind it."""
+    dy [R][Op]; `n_out`: O, when dy carries padding lanes behind it.  `out_dw` / `out_db` share no memory with each other or with
+    an input."""
     _same_device(dy, q)
+    if out_dw is not None or out_db is not None:
+        _apart("dense_wgrad8", (("out_dw", out_dw), ("out_db", out_db)),
+               (("dy", dy), ("the codes", q.codes), ("the scales", q.scales)))
     return _b(dy).dense_wgrad8(q, dy, out_dw, out_db, n_out)
 
 

@@ -2455,12 +2455,6 @@ def _chk_out(t, n, dtypes, like, name):
         raise ValueError(f"{name}: not 16-byte aligned")
 
 
-def _overlap(a, b):
-    """Two contiguous tensors share memory."""
-    pa, pb = a.data_ptr(), b.data_ptr()
-    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
-
-
 def ceil_div(a, b):
     return -(-a // b)
 
@@ -2487,8 +2481,6 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
     if labels.dtype != torch.int64 or not labels.is_contiguous() or labels.numel() != N:
         raise ValueError(f"labels must be a contiguous int64 vector of {N} class numbers")
     dw = db = dx = None
-    if out_dw is not None and (_overlap(out_dw, w) or _overlap(out_dw, x)):
-        raise ValueError("dense_softmax_ce: out_dw overlaps w or x, which are still read while it is written")
     if want_grad:
         if out_dw is not None:
             grad_dtype = out_dw.dtype

@@ -125,6 +125,28 @@ def test_cpu_refusals():
         F.unpack8(q, out=torch.empty(5))
 
 
+def overlaps(x, dy):
+    """Outputs over an input or over one another."""
+    q = F.pack8(x)
+    R, K, O = x.shape[0], x.shape[1], dy.shape[1]
+    buf = torch.zeros(4 * R * max(K, O) + 4 * O * K + 64, dtype=torch.uint8, device=x.device)
+    codes = buf[:R * K].view(torch.int8).view(R, K)
+    codes.copy_(q.codes)
+    p = F.Packed8(codes, q.scales)
+    d = buf[:dy.numel() * dy.element_size()].view(dy.dtype).view(R, O)
+    flat = buf[:4 * O * K].view(torch.float32)
+    for call in (lambda: F.unpack8(p, out=buf[:R * K * x.element_size()].view(x.dtype).view(R, K)),
+                 lambda: F.dense_wgrad8(p, dy, out_dw=flat.view(O, K)), lambda: F.dense_wgrad8(p, dy, out_db=flat[:O]),
+                 lambda: F.dense_wgrad8(q, d, out_dw=flat.view(O, K)), lambda: F.dense_wgrad8(q, d, out_db=flat[:O]),
+                 lambda: F.dense_wgrad8(q, dy, out_dw=flat.view(O, K), out_db=flat[8:8 + O])):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_cpu_overlapping_outputs_are_refused():
+    overlaps(values(40, 32, 1).float(), values(40, 16, 2).float())
+
+
 # ------------------------------------------------------------------------------------------------ device
 DEV_SHAPES = [(1, 8), (1, 16), (5, 24), (3, 1000), (257, 40), (1000, 264), (4099, 128)]
 
@@ -301,3 +323,8 @@ def test_dense_wgrad8_bad_last_block(tile, R, K, O, col, monkeypatch):
     first = ((R - 1) * K + col) // 32 * 32
     nan[first:first + 32] = True
     assert torch.equal(torch.isnan(dw).cpu(), nan.view(R, K).any(0).expand(O, K)) and torch.isfinite(db).all()
+
+
+@pytest.mark.gpu
+def test_overlapping_outputs_are_refused():
+    overlaps(values(40, 32, 1).cuda(), values(40, 16, 2).cuda())

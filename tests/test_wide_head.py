@@ -151,6 +151,26 @@ def test_cpu_refusals():
         F.dense_softmax_ce(x, w, None, lab, out_db=torch.empty(80))
 
 
+def overlaps(x, w, b, lab):
+    """Calls whose gradients would land in an input or in one another."""
+    V, K = w.shape
+    flat = torch.zeros(V * K + V, dtype=b.dtype, device=b.device)
+    ints = torch.zeros(2 * V, dtype=torch.int64, device=b.device)
+    ints[:lab.numel()] = lab
+    for args in (dict(out_db=b), dict(bias=flat[8:8 + V], out_db=flat[16:16 + V]), dict(bias=flat[8:8 + V], out_dw=flat[:V * K].view(V, K)),
+                 dict(out_dw=flat[:V * K].view(V, K), out_db=flat[V * K - 8:V * K - 8 + V]),
+                 dict(labels=ints[:lab.numel()], out_db=ints.view(torch.float32)[8:8 + V])):
+        with pytest.raises(ValueError):
+            F.dense_softmax_ce(**{**dict(x=x, w=w, bias=b, labels=lab), **args})
+    dw, db = flat[:V * K].view(V, K), flat[V * K:]            # neighbours are apart
+    F.dense_softmax_ce(x, w, b, lab, out_dw=dw, out_db=db)
+
+
+def test_cpu_overlapping_gradients_are_refused():
+    x, w, b, lab = make(8, 16, 80)
+    overlaps(x.float(), w.float(), b, lab)
+
+
 def test_scored_rows_come_in_pieces_a_launch_can_hold():
     """A piece's launches hold less than 2^32 threads (256 per row, 256 per 128 statistics of 8 bytes), so its workspace stops
     growing: at 2^20 rows, and at 4 GiB of statistics however much the caller allows."""
@@ -510,3 +530,8 @@ def test_scoring_more_rows_than_a_launch_holds(N, K):
     ref = exact(*a)
     check((loss, None, None, None, rows[:64]), ref)
     assert torch.equal(rows.view(-1, 64), rows[:64].expand(N // 64, 64))
+
+
+@pytest.mark.gpu
+def test_overlapping_gradients_are_refused():
+    overlaps(*cuda(*make(8, 16, 80)))
