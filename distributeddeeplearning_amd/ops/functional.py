@@ -298,13 +298,16 @@ def _cpu_out(t, out, dtype):
 # 8-bit activation checkpoints ----------------------------------------------------------------
 class Packed8:
     """An activation tensor in 8 bits: `codes` (int8, the tensor's shape) and `scales` (uint8, one per 32 consecutive
-    codes in memory order, exponent + 127; 255: the block held a NaN or an infinity and reads as NaN).  The value of a
-    code is code * 2^(scale - 127), exact in bf16."""
+    codes in memory order, exponent + 127, 8 to 248; 255: the block held a NaN or an infinity and reads as NaN).  The value
+    of a code is code * 2^(scale - 127), exact in bf16.  Both are contiguous: a block is 32 neighbours in memory, which a copy of
+    a transposed view would take apart."""
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
             raise ValueError(f"Packed8: int8 codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("Packed8: codes and scales have to be contiguous")
         if scales.numel() != (codes.numel() + 31) // 32:
             raise ValueError(f"Packed8: {codes.numel()} codes need {(codes.numel() + 31) // 32} scales, got {scales.numel()}")
         self.codes, self.scales = codes, scales

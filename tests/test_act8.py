@@ -125,6 +125,17 @@ def test_cpu_refusals():
         F.unpack8(q, out=torch.empty(5))
 
 
+def test_cpu_codes_in_another_order_are_refused():
+    """Scales belong to 32 neighbours in memory: transposed codes would be unpacked, or copied by a reshape, with the scales of
+    other elements."""
+    q = F.pack8(values(64, 40, 3, 20.0).float())
+    for codes, scales in ((q.codes.t(), q.scales), (q.codes.view(64, 5, 8).transpose(1, 2), q.scales),
+                          (q.codes, q.scales.repeat_interleave(2)[::2])):
+        with pytest.raises(ValueError):
+            F.Packed8(codes, scales)
+    assert same(F.unpack8(q.reshape(40, 64)).reshape(-1), F.unpack8(q).reshape(-1))
+
+
 def overlaps(x, dy):
     """Outputs over an input or over one another."""
     q = F.pack8(x)
