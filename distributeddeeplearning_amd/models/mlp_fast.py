@@ -88,10 +88,10 @@ def _chain(net):
 
 def eligible(model) -> bool:
     """Can this RandomModel be trained by the persistent kernel?  (device MLP chain within the kernel's limits,
-    cross-entropy loss, no data parallelism, dataset of 1-channel uint8 images)."""
+    cross-entropy loss, no data parallelism, no 8-bit activations, dataset of 1-channel uint8 images)."""
     net = model.net
-    if not (net.on_gpu and model.dp is None and model.averager is None):
-        return False
+    if not (net.on_gpu and model.dp is None and model.averager is None) or net.keep8:
+        return False                        # (the kernel keeps its activations in LDS, in fp32: nothing to keep in 8 bits)
     if model.loss_name != "categorical_crossentropy" or model.opt.cfg.kind not in _OPT:
         return False
     chain = _chain(net)

@@ -288,3 +288,34 @@ def test_softmax_of_more_wide_rows_than_a_launch_holds():
     assert torch.equal(all_.view(-1, 64, 65), one.expand(B // 64, 64, 65))
     ref = torch.softmax(z[:, :65].double(), 1)
     assert ((one.double() - ref).abs() <= 2.0 ** -15 * ref).all()
+
+
+def mlp_member(device, keep8, seed=0):
+    """A member inside the persistent MLP kernel's limits (32 units, batches of 32)."""
+    sp = config.get_space("ddl_ray", ["data_train_size=250", f"keep8={keep8}", "epochs=2", "mini_epochs=2"])
+    data = Data(device, channels=1, n_train=300, n_test=40, synthetic=True)
+    m = spec(ir.Flatten("f"), ir.Dense("d1", 24, "relu"), ir.Dense("d2", 32, "tanh"), ir.Dense("o", 10, "softmax"),
+             shape=data.input_shape)
+    cs = search.CompiledSpec(m, OptimConfig.keras("adam", 1e-3), "categorical_crossentropy")
+    return RandomModel(data, data.get_random_sample(250, seed=seed), sp, cs, device, 0, seed=seed, verbose=False)
+
+
+def test_persistent_kernel_leaves_keep8_members_alone(monkeypatch):
+    """Its activations are fp32 in LDS: a member that keeps 8 bits would train differently in a group than alone."""
+    from distributeddeeplearning_amd.models import mlp_fast
+    for keep8 in (0, 1):
+        m = mlp_member("cpu", keep8)
+        monkeypatch.setattr(m.net, "on_gpu", True)
+        monkeypatch.setattr(next(op for op in m.net.ops if isinstance(op, ConvOp)), "kstruct", (28, 28, 1))
+        assert mlp_fast.eligible(m) == (not keep8)
+
+
+@pytest.mark.gpu
+def test_keep8_members_train_alike_alone_and_side_by_side():
+    from distributeddeeplearning_amd.models import mlp_fast
+    from distributeddeeplearning_amd.models.classifier import train_concurrently
+    alone, a, b = (mlp_member("cuda", 1, s) for s in (0, 0, 1))
+    assert mlp_fast.eligible(mlp_member("cuda", 0)) and not mlp_fast.eligible(a)
+    alone.train()
+    train_concurrently([a, b])
+    assert a.history == alone.history and torch.equal(a.net.P, alone.net.P)
