@@ -319,6 +319,10 @@ class RandomModel:
             outs.append(F.softmax(y, self.net.out_shape[-1]))
         return torch.cat(outs, 0)
 
+    def test_data(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(images, targets) of the resident test split; class numbers where the head is wider than the one-hot rows."""
+        return self.data.test_x, self.data.test_labels if self._wide else self.data.test_y
+
     def get_accuracy(self, validation_data: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> float:
         self.sync_bn_stats()
         if validation_data is None:

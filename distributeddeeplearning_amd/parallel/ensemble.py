@@ -73,7 +73,7 @@ class MemberActor:
 
     def get_accuracy(self, on_test: bool = False) -> float:
         if on_test:
-            return self.model.get_accuracy((self.data.test_x, self.data.test_y))
+            return self.model.get_accuracy(self.model.test_data())
         return self.model.get_accuracy()
 
     def predict_test(self) -> np.ndarray:

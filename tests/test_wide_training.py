@@ -319,3 +319,30 @@ def test_keep8_members_train_alike_alone_and_side_by_side():
     alone.train()
     train_concurrently([a, b])
     assert a.history == alone.history and torch.equal(a.net.P, alone.net.P)
+
+
+def actor(device, classes):
+    from distributeddeeplearning_amd.parallel.ensemble import MemberActor
+    sp = config.get_space("ddl_ray", ["data_train_size=250", "channels=1"])
+    m = spec(ir.Flatten("f"), ir.Dense("d1", 24, "relu"), ir.Dense("o", classes, "softmax"), shape=(28, 28, 1))
+    cs = search.CompiledSpec(m, OptimConfig.keras("adam", 1e-3), "categorical_crossentropy")
+    return MemberActor(sp, cs, 0, 0, 0, data_kw=dict(n_train=300, n_test=40, synthetic=True), device=device, verbose=False)
+
+
+def check_actor(device):
+    """The test accuracy of a hosted member, against its own predictions: wide heads by class numbers, the others by their
+    one-hot rows."""
+    for classes in (10, 100):
+        a = actor(device, classes)
+        want = int((torch.from_numpy(a.predict_test()).argmax(1) == a.data.test_labels.cpu()).sum()) / 40
+        assert a.get_accuracy(True) == want
+        assert a.model.test_data()[1].dim() == (1 if classes > 64 else 2)
+
+
+def test_hosted_member_of_any_width_is_tested_cpu():
+    check_actor("cpu")
+
+
+@pytest.mark.gpu
+def test_hosted_member_of_any_width_is_tested():
+    check_actor("cuda")
