@@ -846,11 +846,13 @@ class _Keep8:
     def __init__(self, x):
         self.x, self.q, self.held = x, None, True
 
-    def after(self, op, y):
+    def after(self, op, out, y):
+        """`out`: what the op returned; `y`: that as the next op gets it (the oracle rounds to bf16 in between, and it is the
+        rounded tensor that a device packs)."""
         if isinstance(op, ViewOp):
             self.x, self.q = y, None if self.q is None else self.q.reshape(*y.shape)
             return
-        out = []
+        packed = []
 
         def pack_x():
             if self.q is None and not self.held:
@@ -858,13 +860,13 @@ class _Keep8:
             return self.q
 
         def pack_y():
-            if not out:
-                out.append(F.pack8(y))
-            return out[0]
+            if not packed:
+                packed.append(F.pack8(y))
+            return packed[0]
         kept = op.keep8(pack_x, pack_y)
-        same = y is self.x              # the op passed its input on (a BatchNorm its neighbour applies)
+        same = out is self.x            # the op passed its input on (a BatchNorm its neighbour applies)
         self.held = not kept or (same and self.held)
-        self.q = out[0] if out else (self.q if same else None)
+        self.q = packed[0] if packed else (self.q if same else None)
         self.x = y
 
 
@@ -1214,12 +1216,12 @@ class Network:
         try:
             keep = _Keep8(x) if training and self.keep8 else None
             for op in self.ops[start:stop]:
-                x = op.fwd(x, training)
-                if keep is not None:
-                    keep.after(op, x)
+                y = x = op.fwd(x, training)
                 if self.emulate_bf16 and not self.on_gpu and not isinstance(op, ViewOp) \
                         and not (training and getattr(op, "fp32_handoff", False)):
                     x = x.bfloat16().float()
+                if keep is not None:
+                    keep.after(op, y, x)
         finally:
             if out is not None:
                 last.out_buffer = None

@@ -195,3 +195,21 @@ def test_keep8_lowers_the_peak_of_a_batchnorm_network():
     off, on = (peak_of_a_step(m, k, 128, shape) for k in (False, True))
     print(f"peak {off / A:.2f} A in bf16, {on / A:.2f} A in 8 bits")
     assert on <= off - (2 * layers - 1) * A * 31 // 64 + 3 * A        # (the first layer's input is the network's: not packed)
+
+
+def test_the_oracle_packs_what_a_device_packs():
+    """A device packs bf16 tensors: the bf16-emulating oracle packs after its rounding, not before."""
+    seen = []
+
+    def spy(x):
+        seen.append(torch.equal(x, x.bfloat16().float()))
+        return pack(x)
+    pack, F.pack8 = F.pack8, spy
+    try:
+        for m in (conv_net(), padded_net()):
+            net = Network(m, "cpu", seed=1)
+            net.keep8 = net.emulate_bf16 = True
+            net.forward(net.prepare_input(images(4)), training=True)
+    finally:
+        F.pack8 = pack
+    assert len(seen) > 10 and all(seen)
