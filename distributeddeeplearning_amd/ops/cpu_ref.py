@@ -234,6 +234,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad: bool = True):
         raise ValueError(f"labels must be an int64 vector of {N} class numbers")
     if bias is not None and bias.numel() != V:
         raise ValueError(f"bias: {bias.numel()} elements, need {V}")
+    labels = labels.reshape(-1)                # a column of them too, as on the device
     live = (labels >= 0) & (labels < V)
     count = (labels >= 0).sum().clamp_min(1).float()
     xf = torch.where(live[:, None], x.float(), torch.zeros(()))

@@ -135,6 +135,16 @@ def test_cpu_rows_without_label_and_bad_labels():
     assert (dx[0] == 0).all() and torch.isfinite(dw).all()
 
 
+def check_label_column(x, w, b, lab):
+    one, two = F.dense_softmax_ce(x, w, b, lab), F.dense_softmax_ce(x, w, b, lab[:, None])
+    assert all(p.shape == q.shape and torch.equal(p, q) for p, q in zip(one, two))
+
+
+def test_cpu_labels_in_a_column():
+    x, w, b, lab = make(7, 16, 80, drop=0.3)
+    check_label_column(x.float(), w.float(), b, lab)
+
+
 def test_cpu_refusals():
     x, w, b, lab = make(4, 16, 80)
     x, w = x.float(), w.float()
@@ -535,3 +545,8 @@ def test_scoring_more_rows_than_a_launch_holds(N, K):
 @pytest.mark.gpu
 def test_overlapping_gradients_are_refused():
     overlaps(*cuda(*make(8, 16, 80)))
+
+
+@pytest.mark.gpu
+def test_labels_in_a_column():
+    check_label_column(*cuda(*make(7, 16, 80, drop=0.3)))
