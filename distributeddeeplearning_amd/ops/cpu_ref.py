@@ -254,7 +254,7 @@ def dense_softmax_ce(x, w, bias, labels, want_grad: bool = True):
     dl.scatter_add_(1, at, torch.full_like(at, -1, dtype=dl.dtype))
     dl = torch.where(bad[:, None], torch.full_like(dl, math.nan), dl / count)
     dl = torch.where(live[:, None], dl, torch.zeros(()))
-    return loss, dl @ wf, dl.t() @ xf, (dl.sum(0) if bias is not None else None), rows
+    return loss, (dl @ wf).to(x.dtype), dl.t() @ xf, (dl.sum(0) if bias is not None else None), rows
 
 
 # --------------------------------------------------------------------------- 8-bit activation checkpoints

@@ -145,6 +145,13 @@ def test_cpu_labels_in_a_column():
     check_label_column(x.float(), w.float(), b, lab)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_cpu_input_gradient_has_the_inputs_type(dtype):
+    x, w, b, lab = make(5, 16, 80)
+    a, ref = F.dense_softmax_ce(x.to(dtype), w.float(), b, lab)[1], F.dense_softmax_ce(x.float(), w.float(), b, lab)[1]
+    assert a.dtype == dtype and torch.equal(a, ref.to(dtype))
+
+
 def test_cpu_refusals():
     x, w, b, lab = make(4, 16, 80)
     x, w = x.float(), w.float()
