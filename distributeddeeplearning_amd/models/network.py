@@ -1338,11 +1338,11 @@ class Network:
         layers that ran with batch groups, the statistics of `group`): the following backward then differentiates
         that part of the batch alone.  Used when one forward serves two purposes -- the DCGAN generator runs ONCE
         on [z1 ; z2] per step, the first half feeds the discriminator phase, only the second half is trained."""
+        if any(isinstance(getattr(op, attr, None), F.Packed8) for op in self.ops for attr in ("x", "y")):
+            raise ValueError("narrow_saved: the activations were kept in 8 bits (Network.keep8)")
         for op in self.ops:
             for attr in ("x", "y", "x_img"):
                 t = getattr(op, attr, None)
-                if isinstance(t, F.Packed8):
-                    raise ValueError("narrow_saved: the activations were kept in 8 bits (Network.keep8)")
                 if isinstance(t, torch.Tensor) and t.dim() >= 1:
                     setattr(op, attr, t[lo:hi])
             if isinstance(op, BNOp) and op.mean is not None and op.groups_used > 1:

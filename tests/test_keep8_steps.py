@@ -213,3 +213,13 @@ def test_the_oracle_packs_what_a_device_packs():
     finally:
         F.pack8 = pack
     assert len(seen) > 10 and all(seen)
+
+
+def test_a_refused_narrowing_changes_nothing():
+    net = Network(conv_net(), "cpu", seed=1)
+    net.keep8 = True
+    y = net.forward(net.prepare_input(images(6)), training=True)
+    with pytest.raises(ValueError):
+        net.narrow_saved(0, 3)
+    assert net.ops[0].x.shape[0] == 6
+    assert net.backward(torch.ones_like(y), need_input_grad=True).shape[0] == 6
