@@ -27,8 +27,8 @@ OBJ = ROOT / "build" / "obj"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 HIPCC = str(ROCM / "bin" / "hipcc")
 ARCH = "gfx950"
-# no packed fp32 instructions: some of their forms have given wrong results on this hardware (hipcc -O3 makes them by
-# itself; the host pass warns that it does not know the feature)
+# no packed fp32 instructions (hipcc -O3 makes them by itself): a precaution, every kernel is tested and measured without them;
+# the host pass warns that it does not know the feature
 NO_PK_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -15,7 +15,7 @@ Design (MI355X-first, not a Keras clone):
   * no autograd: every op has a hand-written backward that calls the HIP kernels;
   * what a training forward keeps for the backward pass is bf16, or with `Network.keep8` 8 bits (ops/functional.py
     pack8) wherever no fused kernel wants the bf16 tensor;
-  * a softmax head of any width trains and scores from integer labels without its logits (`Network.train_labels`,
+  * a softmax head of any width trains and scores from integer labels and keeps no logits (`Network.train_labels`,
     `Network.score`).
 
 Replaces what Keras' `Model`/`fit` machinery did for the reference (/root/reference/DDL.py:58-96,
@@ -1367,7 +1367,7 @@ class Network:
     def train_labels(self, x, labels):
         """Forward and backward of the categorical cross-entropy of a softmax Dense head of any width against class numbers
         (`labels` int64, negative: sample left out): the head's logits, their gradient and its own weight gradient are
-        one operator that never holds the logits (F.dense_softmax_ce).  Gradients land in `self.G`; returns (mean loss,
+        one operator that does not keep the logits (F.dense_softmax_ce).  Gradients land in `self.G`; returns (mean loss,
         sample losses).  `x` as prepare_input leaves it."""
         op = self._label_head()
         h = self.forward(x, training=True, stop=-1)

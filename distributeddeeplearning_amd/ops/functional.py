@@ -259,7 +259,8 @@ def _apart(what, outs, ins):
 
 
 def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):
-    """Dense(K -> V) + softmax cross entropy for any number of classes, forward and backward, without the logits.
+    """Dense(K -> V) + softmax cross entropy for any number of classes, forward and backward.  The logits are not kept; on the
+    device a step keeps their exponentials, 2 bytes per row and class, at most DDL_CE_PIECE_BYTES (4 GiB) of them at a time.
 
     x [N][K], w [V][K] (device: bf16, K padded to a multiple of 8 with zero lanes), bias [V] fp32 or None (-inf switches
     a class off; on the device so does anything below -2.3e38, the type's lowest value among it), labels [N] int64.  A row
@@ -270,7 +271,8 @@ def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=Non
 
     A label past the last class makes its row loss (and the mean) NaN and its row no gradient; a labelled row with a NaN
     or infinite logit, or with every class switched off, has NaN loss and gradients.  On the device the gradient of the
-    logits is rounded to bf16 as every dY is, twice for dw (its scale is folded into x)."""
+    logits is rounded to bf16 as every dY is, twice for dw (its scale is folded into x), the label's own entry excepted: fp32
+    gradients are good to 5e-5 .. 4e-4 of their rms, not to fp32's 1e-7.  The losses are fp32 throughout."""
     if out_dw is not None or out_db is not None:
         _apart("dense_softmax_ce", (("out_dw", out_dw), ("out_db", out_db)),
                (("x", x), ("w", w), ("bias", bias), ("labels", labels)))
