@@ -245,17 +245,20 @@ def _apart(what, outs, ins):
     """Refuse outputs that share memory with an input or with one another: kernels write outputs while others still read (a
     gradient over the bias would be the next piece of rows' bias).  (name, tensor or None) each; contiguous ones, as the device
     wants them."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-    done = [(n, *span(t)) for n, t in ins if t is not None and t.numel() and t.is_contiguous()]
+    spans = []
+    for name, t in ins:
+        if t is not None:
+            lo = t.data_ptr()
+            spans.append((lo, lo + t.nbytes, name, t))
     for name, t in outs:
-        if t is None or not t.numel() or not t.is_contiguous():
+        if t is None:
             continue
-        lo, hi = span(t)
-        for other, a, b in done:
-            if lo < b and a < hi:
+        lo = t.data_ptr()
+        hi = lo + t.nbytes
+        for a, b, other, u in spans:
+            if lo < b and a < hi and a < b and lo < hi and t.is_contiguous() and u.is_contiguous():
                 raise ValueError(f"{what}: {name} overlaps {other}")
-        done.append((name, lo, hi))
+        spans.append((lo, hi, name, t))
 
 
 def dense_softmax_ce(x, w, bias, labels, want_grad=True, out_dw=None, out_db=None, grad_dtype=torch.float32):

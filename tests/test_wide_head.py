@@ -179,8 +179,10 @@ def overlaps(x, w, b, lab):
                  dict(labels=ints[:lab.numel()], out_db=ints.view(torch.float32)[8:8 + V])):
         with pytest.raises(ValueError):
             F.dense_softmax_ce(**{**dict(x=x, w=w, bias=b, labels=lab), **args})
-    dw, db = flat[:V * K].view(V, K), flat[V * K:]            # neighbours are apart
+    dw, db = flat[:V * K].view(V, K), flat[V * K:]            # neighbours are apart, and so is a batch of no rows inside one
     F.dense_softmax_ce(x, w, b, lab, out_dw=dw, out_db=db)
+    none = flat.view(x.dtype)[64:64].view(0, K)
+    F.dense_softmax_ce(none, w, b, lab[:0], out_dw=dw, out_db=db)
 
 
 def test_cpu_overlapping_gradients_are_refused():
