@@ -401,7 +401,7 @@ class ConvOp(Op):
                     else:
                         hip.conv_wgrad(x, d, g1, "A", out=self.gkernel, x_affine=xa)
                         self._bias_grad(dy)
-                _BR.run(wg, dy)
+                _BR.run(wg, dy, x, dyc[0])      # (both may be tensors of this call, made on the main stream)
         return dx
 
     def _fwd_up(self, x, training):
@@ -495,7 +495,7 @@ class ConvOp(Op):
                                                                g, self.gkernel, bn=bnd, fwdconv=self.onech == "in")
                     if done[0]:
                         self._bias_grad(dy)
-                _BR.run(wg_up, dy)
+                _BR.run(wg_up, dy, bnd)         # (bnd's coefficients: main-stream tensors that only it holds)
                 if done[0]:
                     return None
             if bnd is not None:         # (not reached with the shipped shapes) the generic kernels want the real dx

@@ -223,3 +223,38 @@ def test_a_refused_narrowing_changes_nothing():
         net.narrow_saved(0, 3)
     assert net.ops[0].x.shape[0] == 6
     assert net.backward(torch.ones_like(y), need_input_grad=True).shape[0] == 6
+
+
+def test_branch_keeps_the_taps_and_coefficients_of_one_channel_layers(monkeypatch):
+    """The taps tensor of dY (a layer with one output channel) and the coefficients of a BatchNorm applied on load (a layer with
+    one input channel) are made on the main stream and read by the branch: held until the join."""
+    kept, fresh = [], []
+
+    def branch(fn, *keep):
+        kept.extend(keep)
+        fn()
+
+    class Kernels:
+        tapconv_1ch = staticmethod(lambda *a, **k: None)
+        conv_dgrad = staticmethod(lambda dy, *a, **k: dy)
+        conv_wgrad = staticmethod(lambda *a, **k: None)
+        upconv_1ch_wgrad = staticmethod(lambda *a, **k: True)
+
+        @staticmethod
+        def im2col_1ch(img, g, **k):
+            fresh.append(torch.zeros(2, g.OH, g.OW, 16))
+            return fresh[-1]
+    monkeypatch.setattr(network._BR, "run", branch)
+    monkeypatch.setattr(F, "hip_backend", lambda: Kernels)
+    net = Network(spec(ir.Conv2DTranspose("t", 1, (3, 3), 1, 1, "same"), shape=(8, 8, 4)), "cpu")
+    op = net.ops[0]
+    op.onech, op.g1, op.w_tapT = "out", op.g, torch.zeros(9, 4)
+    op.x = torch.zeros(2, 8, 8, 4)
+    monkeypatch.setattr(op, "_bias_grad", lambda dy: None)
+    op._bwd_onech(torch.zeros(2, 8, 8, 1), True, True)
+    assert len(fresh) == 1 and any(t is fresh[0] for t in kept) and any(t is op.x for t in kept)
+    kept.clear()
+    op.onech, op.bn_deferred, coefficients = "up", {}, torch.zeros(4)
+    op.bn_deferred["c1"] = coefficients
+    op.bwd(torch.zeros(2, 8, 8, 1), need_dx=False)
+    assert any(isinstance(t, dict) and t["c1"] is coefficients for t in kept)
